@@ -14,13 +14,19 @@ Public entry points:
 * ``set_sm_limit(n)`` / ``sm_limit(n)``: cap the SMs the persistent kernels
   use, leaving the rest to kernels of other streams (NCCL collectives of a
   sharded pipeline, ``shard.attention_by_rows_pipelined``).
+* ``attn_cache4(q, cache, ...)``: attention of a few or many new tokens per
+  request against a paged key/value cache held in 4 bits, with
+  ``cache4_alloc``, ``cache4_plan`` (page tables and slots, on the GPU),
+  ``cache4_write`` and ``cache4_read`` (``cache4.py``).
 """
 
 import contextlib
 
+from .cache4 import Cache4Plan, attn_cache4, cache4_alloc, cache4_plan, cache4_read, cache4_write
 from .gfx906_attn import is_sm100, last_error, load_attention
 
-__all__ = ["attn", "attn_dmajor", "attn_host", "device_status", "is_sm100", "load_attention", "last_error",
+__all__ = ["Cache4Plan", "attn", "attn_cache4", "attn_dmajor", "attn_host", "cache4_alloc", "cache4_plan",
+           "cache4_read", "cache4_write", "device_status", "is_sm100", "load_attention", "last_error",
            "set_sm_limit", "sm_limit"]
 
 

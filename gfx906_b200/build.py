@@ -3,12 +3,13 @@
 Two artefacts are built next to this file, so that they travel with the
 source tree and no JIT cache is involved:
 
-* ``libgfx906_b200_attn.so``: the C-ABI library (``include/gfx906_b200_attn.h``),
-  compiled by nvcc for ``sm_100a`` only. It has no torch dependency; this is
+* ``libgfx906_b200_attn.so``: the C-ABI library (``include/gfx906_b200_attn.h``,
+  ``include/gfx906_b200_cache4.h``), compiled by nvcc for ``sm_100a`` only. It has no torch dependency; this is
   the object the reference's ``attn.cpp`` links against (the reference links
   ``attn_kernel.gfx906.o`` the same way, ``deploy/gfx906_attn.py:78-83``).
-* ``_attn_ext<EXT_SUFFIX>``: the torch operator (``csrc/attn.cpp``), a pybind11
-  module exposing ``attn(q, k, v, scale)``, linked to the library above.
+* ``_attn_ext<EXT_SUFFIX>``: the torch operators (``csrc/attn.cpp``,
+  ``csrc/cache4.cpp``), a pybind11 module exposing ``attn(q, k, v, scale)`` and
+  the operators of the 4-bit cache, linked to the library above.
 
 Each artefact is rebuilt only when a hash of its sources, flags and compiler
 changes (stored beside it as ``<artefact>.buildhash``); file modification
@@ -36,8 +37,13 @@ EXT_NAME = "_attn_ext"
 EXT_PATH = PKG_DIR / (EXT_NAME + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 # Every CUDA translation unit of the library.
-CU_SOURCES = [CSRC / "attn_fwd_sm100.cu", CSRC / "attn_fwd_noalloc.cu"]
-CU_HEADERS = [CSRC / "sm100_ptx.cuh", INCLUDE / "gfx906_b200_attn.h"]
+CU_SOURCES = [CSRC / "attn_fwd_sm100.cu", CSRC / "attn_fwd_noalloc.cu", CSRC / "cache4_store.cu",
+              CSRC / "cache4_attn.cu"]
+CU_HEADERS = [CSRC / "sm100_ptx.cuh", CSRC / "cache4.cuh", CSRC / "cache4_attn.cuh", CSRC / "cache4_host.cuh",
+              INCLUDE / "gfx906_b200_attn.h", INCLUDE / "gfx906_b200_cache4.h"]
+# The torch operator module and the headers it shares with the library.
+EXT_SOURCES = [CSRC / "attn.cpp", CSRC / "cache4.cpp"]
+EXT_HEADERS = [INCLUDE / "gfx906_b200_attn.h", INCLUDE / "gfx906_b200_cache4.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -127,12 +133,11 @@ def build_extension(force: bool = False) -> Path:
     lib = build_library(force=force)
     cflags, ldflags, tver = _torch_flags()
     cxx = os.environ.get("CXX", "g++")
-    src = CSRC / "attn.cpp"
-    digest = _digest([src, INCLUDE / "gfx906_b200_attn.h", lib], cflags + ldflags + [tver, cxx])
+    digest = _digest([*EXT_SOURCES, *EXT_HEADERS, lib], cflags + ldflags + [tver, cxx])
     if not force and _fresh(EXT_PATH, digest):
         return EXT_PATH
     tmp = EXT_PATH.with_name(EXT_PATH.name + ".tmp")
-    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", str(src), "-o", str(tmp), *cflags,
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", *map(str, EXT_SOURCES), "-o", str(tmp), *cflags,
            f"-L{PKG_DIR}", "-lgfx906_b200_attn", "-Wl,-rpath,$ORIGIN", *ldflags]
     _run(cmd, PKG_DIR / ".cxx.log")
     os.replace(tmp, EXT_PATH)

@@ -1,4 +1,5 @@
-"""ctypes binding of the C-ABI library (``include/gfx906_b200_attn.h``).
+"""ctypes binding of the C-ABI library (``include/gfx906_b200_attn.h``,
+``include/gfx906_b200_cache4.h``).
 
 This is the stub a host application without torch would write to call the
 library; the tests use it to check the exported surface and to drive the
@@ -14,6 +15,17 @@ STATUS = {"OK": 0, "EINVAL": 1, "EHEADDIM": 2, "EALIGN": 3, "ENODEV": 4, "ECUDA"
           "ENOSPACE": 7}
 
 _c_int, _c_void_p, _c_float = ctypes.c_int, ctypes.c_void_p, ctypes.c_float
+_c_ll = ctypes.c_longlong
+
+
+class Cache4AttnArgs(ctypes.Structure):
+    """``gfx906_b200_cache4_attn_args``."""
+
+    _fields_ = [(name, _c_void_p) for name in ("q", "o", "cache", "tables", "lengths", "query_start", "k_scale",
+                                               "v_scale")] + \
+               [(name, _c_ll) for name in ("q_stride_t", "q_stride_h", "o_stride_t", "o_stride_h")] + \
+               [(name, _c_int) for name in ("dtype", "tokens", "heads", "kv_heads", "D", "pages", "requests", "width",
+                                            "max_tokens", "causal", "zero_rest")] + [("scale", _c_float)]
 
 
 class CABI:
@@ -50,6 +62,19 @@ class CABI:
         d.gfx906_b200_attn_set_sm_limit.argtypes, d.gfx906_b200_attn_set_sm_limit.restype = [_c_int], _c_int
         d.gfx906_b200_attn_flops.argtypes = [_c_int] * 5
         d.gfx906_b200_attn_flops.restype = ctypes.c_double
+        d.gfx906_b200_cache4_page_bytes.argtypes, d.gfx906_b200_cache4_page_bytes.restype = [_c_int], _c_int
+        d.gfx906_b200_cache4_plan.argtypes = [_c_void_p] * 5 + [_c_int] * 4 + [_c_void_p] * 7
+        d.gfx906_b200_cache4_plan.restype = _c_int
+        d.gfx906_b200_cache4_write.argtypes = [_c_void_p] * 2 + [_c_int] + [_c_ll] * 4 + [_c_int] * 3 + \
+            [_c_void_p, _c_int] + [_c_void_p] * 4
+        d.gfx906_b200_cache4_write.restype = _c_int
+        d.gfx906_b200_cache4_read.argtypes = [_c_void_p, _c_int] + [_c_void_p] * 3 + [_c_int] * 3 + \
+            [_c_void_p] * 2 + [_c_int, _c_void_p]
+        d.gfx906_b200_cache4_read.restype = _c_int
+        d.gfx906_b200_cache4_attn_workspace_size.argtypes = [ctypes.POINTER(Cache4AttnArgs)]
+        d.gfx906_b200_cache4_attn_workspace_size.restype = ctypes.c_size_t
+        d.gfx906_b200_cache4_attn.argtypes = [ctypes.POINTER(Cache4AttnArgs), _c_void_p, ctypes.c_size_t, _c_void_p]
+        d.gfx906_b200_cache4_attn.restype = _c_int
 
     def launch_status(self, q, k, v, o, B, H, Sq, Skv, D, scale, stream=None) -> int:
         return self.dll.gfx906_b200_attn_launch(q, k, v, o, B, H, Sq, Skv, D, _c_float(scale), stream)

@@ -145,10 +145,13 @@ int64_t set_sm_limit(int64_t sms) {
   return gfx906_b200_attn_set_sm_limit(static_cast<int>(sms));
 }
 
+void register_cache4(pybind11::module_& m);  // cache4.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn", &attn, "flash-attention forward (fp16 [B,H,S,D], sm_100a)");
   m.def("attn_out", &attn_out, "flash-attention forward into a given contiguous fp16 output tensor");
   m.def("attn_dmajor", &attn_dmajor, "flash-attention forward on transposed [B,H,D,S] fp16, D = 512");
   m.def("device_status", &device_status, "device status word (0 = ok)", pybind11::arg("reset") = false);
   m.def("set_sm_limit", &set_sm_limit, "cap on the SMs the persistent kernels use (0 = all); returns the previous");
+  register_cache4(m);
 }

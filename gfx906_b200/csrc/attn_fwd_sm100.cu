@@ -2177,6 +2177,17 @@ int gfx906_b200_internal_set_last_error(int status) {
   return status;
 }
 
+// The current device's checks and the SMs a launch may plan for, for the other
+// translation units of the library.
+int gfx906_b200_internal_device(int* num_sms) {
+  int dev = 0;
+  const int rc = check_device(&dev);
+  if (rc == GFX906_B200_OK) *num_sms = device_sms(dev);
+  return rc;
+}
+
+unsigned long long gfx906_b200_internal_timeout_ns(void) { return timeout_ns_from_env(); }
+
 int gfx906_b200_attn_launch_ws(const void* q, const void* k, const void* v, void* o, int B, int H, int Sq,
                                int Skv, int D, float scale, void* workspace, size_t workspace_bytes,
                                cudaStream_t stream) {
@@ -2198,7 +2209,7 @@ const char* gfx906_b200_attn_error_string(int status) {
   switch (status) {
     case GFX906_B200_OK: return "ok";
     case GFX906_B200_EINVAL: return "invalid argument (negative size, null pointer or size overflow)";
-    case GFX906_B200_EHEADDIM: return "unsupported head_dim (need <=64 and a multiple of 8, 128, or 512)";
+    case GFX906_B200_EHEADDIM: return "unsupported head_dim (need <=64 and a multiple of 8, 128, or 512; the 4-bit cache 64 or 128)";
     case GFX906_B200_EALIGN: return "q, k, v and o must be 16-byte aligned";
     case GFX906_B200_ENODEV: return "current CUDA device is not an sm_100 (B200) GPU";
     case GFX906_B200_ECUDA: return "a CUDA runtime or driver call failed";

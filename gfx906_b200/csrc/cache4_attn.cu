@@ -1,0 +1,746 @@
+// Attention of a few new tokens per request against the paged 4-bit cache
+// (cache4.cuh): O = softmax(scale * q K^T) V over a request's pages.
+//
+// Work is the list of units (request, row tile, kv head): a row tile is 8 * NT
+// query rows of the request, a row being one (token, head of the group), so
+// that all query heads of a kv head share one read of its keys and values. A
+// unit's key range is cut into steps of 32 tokens (half a page, one contiguous
+// copy of 36 D bytes). The steps of all units form one line that the blocks
+// share evenly, whatever the requests' lengths; a unit that is cut at a block's
+// end leaves partial sums (m, l, unnormalised O, 32 bits) in the workspace,
+// joined by cache4_join_kernel. Every unit counts one step more than it has
+// keys for, so that units without any key have an owner that writes their
+// zeros, and as the price of starting a unit.
+//
+// Inside a block four warps take the steps in turn, each with its own ring of
+// copies in flight and its own running maximum m, sum l and accumulator; they
+// meet once per unit. A warp computes S^T = K Q^T and O^T = V^T P^T: the keys
+// and channels fill the 16 rows of m16n8k16 and the query rows are its n, so
+// eight rows (all heads of a group for one token) leave no half of the
+// instruction empty. Codes become fp16 by one conversion and one exact product
+// per pair, in registers.
+#include <limits.h>
+#include <math.h>
+
+#include "cache4.cuh"
+#include "cache4_attn.cuh"
+#include "cache4_host.cuh"
+#include "sm100_ptx.cuh"
+
+namespace c4 {
+
+constexpr int WARPS = 4;
+constexpr int THREADS = WARPS * 32;
+constexpr int STEP = 32;                // tokens of a step
+constexpr int MAX_CHUNKS = 64;          // of THREADS requests
+constexpr int MIN_STEPS = WARPS;        // fewest steps a block is started for
+constexpr int RECORD_INTS = 8;
+
+struct JoinRecord {  // written by the block that starts a cut unit
+  int pieces;        // 0: nothing to join
+  int first;         // first token of the request
+  int row0, rows;    // query rows of the unit
+  int head;          // kv head
+  int pad[3];
+};
+static_assert(sizeof(JoinRecord) == RECORD_INTS * 4, "");
+
+struct FewParams {
+  AttnParams a;
+  int max_rows;       // requests with more query rows are another kernel's
+  float* part_o;      // [blocks][2][8 NT][D]
+  float* part_ml;     // [blocks][2][8 NT][2]
+  JoinRecord* record; // [blocks]
+};
+
+template <int D, int NT>
+struct Few {
+  using L = Layout<D>;
+  static constexpr int ROWS = 8 * NT;
+  static constexpr int STEP_BYTES = 2 * L::BLOCK_BYTES;
+  static constexpr int STAGES = NT == 1 ? 2 : 3;  // four or three blocks share an SM
+  static constexpr int LD = D + 4;  // floats of a row in the merge buffer
+  static constexpr int RING = STAGES * STEP_BYTES;
+  static constexpr int Q_OFF = WARPS * RING;
+  static constexpr int Q_BYTES = ROWS * D * 2;
+  static constexpr int ML_OFF = Q_OFF + Q_BYTES;          // [WARPS][ROWS] (m, l)
+  static constexpr int ROWF_OFF = ML_OFF + WARPS * ROWS * 8;  // [ROWS] factors of the rows of q
+  static constexpr int SMEM = ROWF_OFF + ROWS * 4;
+  static_assert(ROWS * LD * 4 <= RING, "a warp's merge buffer is its ring");
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+  return v;
+}
+// W words at a, W = 2 or 4.
+template <int W>
+__device__ __forceinline__ void lds(uint32_t a, uint32_t* v) {
+  if (W == 4)
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(a)
+                 : "memory");
+  else
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+// Steps (plus one) and units of a request; 0 units when it is not ours.
+struct Share {
+  long long weight;  // of the whole request
+  int steps;         // of one unit, with the one extra
+};
+template <int ROWS>
+__device__ __forceinline__ Share share_of(const FewParams& p, int r) {
+  const int n = rows_of(p.a, r).n;
+  const long long rows = static_cast<long long>(n) * p.a.group;
+  if (n == 0 || rows > p.max_rows) return {0, 0};
+  const int steps = (length_of(p.a, r) + STEP - 1) / STEP + 1;
+  return {(rows + ROWS - 1) / ROWS * p.a.kv_heads * steps, steps};
+}
+
+// Per-thread state of one warp's share of a unit.
+template <int D, int NT>
+struct Acc {
+  float o[D / 16][NT][4];  // O^T: channels n D/8 + 2t (+1), query rows 2c, 2c + 1 of tile nt
+  float m[NT][2], l[NT][2];
+};
+
+// One step of 32 tokens (two blocks at `blk`): scores, running softmax, sums.
+// MASK: tokens key0 + 0..31 may lie behind the last one a row sees
+// (limit[nt][i], exclusive) or behind the request's length (`len`): those keys
+// take no part, and their values -- whatever the page holds there -- are zeroed.
+template <int D, int NT, bool MASK>
+__device__ __forceinline__ void step(Acc<D, NT>& acc, uint32_t blk, uint32_t sq, int lane, const float (&factor)[NT][2],
+                                     int key0, int len, const int (&limit)[NT][2]) {
+  using L = Layout<D>;
+  constexpr int W = D / 32;  // words of K codes of a lane and token
+  const int n = lane >> 2, c = lane & 3;
+  float s[2][NT][4];
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[b][nt][e] = 0.f;
+  // ---- S^T = K Q^T
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const uint32_t base = blk + b * L::BLOCK_BYTES;
+    uint32_t k0[W], k1[W];  // tokens n and n + 8
+    lds<W>(base + L::KC + lane * (D / 8), k0);
+    lds<W>(base + L::KC + 4 * D + lane * (D / 8), k1);
+    uint32_t f0[L::GPL], f1[L::GPL];  // scales of tokens n and n + 8, in both halves
+    if (L::GPL == 2) {
+      const uint32_t w = lds32(base + L::KS + lane * 4);
+      const uint32_t x = scales_to_half2(w), y = scales_to_half2(w >> 16);
+      f0[0] = __byte_perm(x, x, 0x1010);
+      f0[L::GPL - 1] = __byte_perm(x, x, 0x3232);
+      f1[0] = __byte_perm(y, y, 0x1010);
+      f1[L::GPL - 1] = __byte_perm(y, y, 0x3232);
+    } else {
+      const uint32_t x = scales_to_half2(lds16(base + L::KS + lane * 2));
+      f0[0] = __byte_perm(x, x, 0x1010);
+      f1[0] = __byte_perm(x, x, 0x3232);
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) {  // two k-steps of 16 channels for each word
+      uint32_t x0[4], x1[4];
+      codes_to_half2(k0[j], x0);
+      codes_to_half2(k1[j], x1);
+      const int g = j * 8 / 16;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x0[e] = mul_half2(x0[e], f0[g]);
+        x1[e] = mul_half2(x1[e], f1[g]);
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        uint32_t qf[4];
+        lds<4>(sq + ((nt * W + j) * 32 + lane) * 16, qf);
+        mma16816(s[b][nt], x0[0], x1[0], x0[1], x1[1], qf[0], qf[1]);
+        mma16816(s[b][nt], x0[2], x1[2], x0[3], x1[3], qf[2], qf[3]);
+      }
+    }
+  }
+  // ---- running softmax; s[b][nt]: tokens 16 b + n (+ 8), rows 2c, 2c + 1
+  uint32_t pb[2][NT][2];
+  float alpha[NT][2];
+  bool grew = false;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = s[b][nt][2 * e + i] * factor[nt][i];
+          if (MASK && key0 + 16 * b + 8 * e + n >= limit[nt][i]) x = -INFINITY;
+          s[b][nt][2 * e + i] = x;
+          mx = fmaxf(mx, x);
+        }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+      const float m_new = fmaxf(acc.m[nt][i], mx);
+      grew |= m_new > acc.m[nt][i];
+      alpha[nt][i] = m_new > acc.m[nt][i] ? fa::ex2_approx(acc.m[nt][i] - m_new) : 1.f;
+      acc.m[nt][i] = m_new;
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;  // no key seen yet
+      float sum = 0.f;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = fa::ex2_approx(s[b][nt][2 * e + i] - m_use);
+          s[b][nt][2 * e + i] = x;
+          sum += x;
+        }
+      acc.l[nt][i] = acc.l[nt][i] * alpha[nt][i] + sum;
+    }
+    // P in fp16 (it is at most 1; the sum keeps 32 bits), transposed into B fragments
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        pb[b][nt][e] = transpose8x8(fa::pack_half2(s[b][nt][2 * e], s[b][nt][2 * e + 1]));
+  }
+  if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        acc.o[t][nt][0] *= alpha[nt][0];
+        acc.o[t][nt][1] *= alpha[nt][1];
+        acc.o[t][nt][2] *= alpha[nt][0];
+        acc.o[t][nt][3] *= alpha[nt][1];
+      }
+  }
+  // ---- O^T += V^T P^T
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const uint32_t base = blk + b * L::BLOCK_BYTES;
+    constexpr int W2 = D / 64;      // words of V codes of a lane and token
+    uint32_t v0[2 * W2], v1[2 * W2];  // tokens 2c, 2c + 1; tokens 2c + 8, 2c + 9
+    lds<2 * W2>(base + L::VC + lane * (D / 8), v0);
+    lds<2 * W2>(base + L::VC + 4 * D + lane * (D / 8), v1);
+    uint32_t w = lds32(base + L::VS + (D == 128 ? lane : (n / 2) * 4 + c) * 4);
+    if (MASK) {
+      const int k = key0 + 16 * b + 2 * c;
+      if (k >= len) w &= 0xffffff00u;
+      if (k + 1 >= len) w &= 0xffff00ffu;
+      if (k + 8 >= len) w &= 0xff00ffffu;
+      if (k + 9 >= len) w &= 0x00ffffffu;
+    }
+    const uint32_t f0 = scales_to_half2(w), f1 = scales_to_half2(w >> 16);
+#pragma unroll
+    for (int j = 0; j < W2; ++j) {
+      // bytes of one channel's codes of two tokens: even channels, odd channels
+      const uint32_t m = 0x0f0f0f0fu;
+      uint32_t e0[4], o0[4], e1[4], o1[4];
+      codes_to_half2((v0[j] & m) | ((v0[W2 + j] & m) << 4), e0);
+      codes_to_half2(((v0[j] >> 4) & m) | (v0[W2 + j] & ~m), o0);
+      codes_to_half2((v1[j] & m) | ((v1[W2 + j] & m) << 4), e1);
+      codes_to_half2(((v1[j] >> 4) & m) | (v1[W2 + j] & ~m), o1);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint32_t a0 = mul_half2(e0[t], f0), a1 = mul_half2(o0[t], f0);
+        const uint32_t a2 = mul_half2(e1[t], f1), a3 = mul_half2(o1[t], f1);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816(acc.o[4 * j + t][nt], a0, a1, a2, a3, pb[b][nt][0], pb[b][nt][1]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ long long range_start(long long total, int blocks, int c) { return total * c / blocks; }
+// The block whose range holds `at`: the largest c with total * c / blocks <= at.
+__device__ __forceinline__ int range_owner(long long at, long long total, int blocks) {
+  return static_cast<int>(((at + 1) * blocks - 1) / total);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void store4(uint16_t* dst, float4 x) {
+  *reinterpret_cast<uint2*>(dst) = make_uint2(float2_to_pair<BF16>(x.x, x.y), float2_to_pair<BF16>(x.z, x.w));
+}
+
+template <int D, int NT, bool BF16>
+__global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) cache4_few_kernel(const FewParams p) {
+  using C = Few<D, NT>;
+  using L = Layout<D>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ long long chunk_before[MAX_CHUNKS + 1];
+  __shared__ long long warp_part[WARPS];
+  __shared__ long long found_base;
+  __shared__ int found_r;
+  const AttnParams& a = p.a;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int n = lane >> 2, c = lane & 3;
+  const uint32_t s0 = fa::smem_u32(smem);
+  const uint32_t ring = s0 + warp * C::RING;
+  float2* ml = reinterpret_cast<float2*>(smem + C::ML_OFF);
+  float* rowf = reinterpret_cast<float*>(smem + C::ROWF_OFF);
+  fa::griddep_wait();
+  if (threadIdx.x == 0) fa::griddep_launch_dependents();
+
+  // ---- this block's part [pos, end) of the line of steps
+  const int chunks = (a.requests + THREADS - 1) / THREADS;
+  long long total = 0;
+  for (int k = 0; k < chunks; ++k) {
+    const int r = k * THREADS + threadIdx.x;
+    long long w = r < a.requests ? share_of<C::ROWS>(p, r).weight : 0;
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) w += __shfl_xor_sync(0xffffffffu, w, d);
+    if (lane == 0) warp_part[warp] = w;
+    __syncthreads();
+    if (threadIdx.x == 0) chunk_before[k] = total;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) total += warp_part[i];
+    __syncthreads();
+  }
+  const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + MIN_STEPS - 1) / MIN_STEPS));
+  JoinRecord rec{};
+  long long pos = 0, end = 0;
+  if (static_cast<int>(blockIdx.x) < blocks) {
+    pos = range_start(total, blocks, blockIdx.x);
+    end = range_start(total, blocks, blockIdx.x + 1);
+  }
+  int r = 0;
+  long long base = 0;
+  if (pos < end) {
+    int k = 0;
+    while (k + 1 < chunks && chunk_before[k + 1] <= pos) ++k;
+    const int rr = k * THREADS + threadIdx.x;
+    const long long w = rr < a.requests ? share_of<C::ROWS>(p, rr).weight : 0;
+    long long inc = w;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const long long y = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += y;
+    }
+    if (lane == 31) warp_part[warp] = inc;
+    __syncthreads();
+    long long before = chunk_before[k] + inc - w;
+    for (int i = 0; i < warp; ++i) before += warp_part[i];
+    if (before <= pos && pos < before + w) {
+      found_base = before;
+      found_r = rr;
+    }
+    __syncthreads();
+    r = found_r;
+    base = found_base;
+  }
+
+  while (pos < end) {
+    const Share sh = share_of<C::ROWS>(p, r);
+    if (pos >= base + sh.weight) {  // the next request (the line ends with the last one's units)
+      base += sh.weight;
+      ++r;
+      continue;
+    }
+    const Rows rows = rows_of(a, r);
+    const int len = length_of(a, r);
+    const long long unit = (pos - base) / sh.steps;
+    const int off = static_cast<int>((pos - base) % sh.steps);
+    const int stop = static_cast<int>(min(static_cast<long long>(sh.steps), off + (end - pos)));
+    const int head = static_cast<int>(unit % a.kv_heads);
+    const int row0 = static_cast<int>(unit / a.kv_heads) * C::ROWS;
+    const int nrows = min(C::ROWS, rows.n * a.group - row0);
+    const int k_begin = max(off, 1) - 1, k_end = stop - 1;  // steps that hold keys
+    const int* table = a.tables + static_cast<long long>(r) * a.width;
+
+    // ---- copies of this warp's first steps
+    int page_ids = 0, ids_at = -32;  // page of step k_begin + warp + WARPS * (ids_at + lane)
+    const int my_steps = k_end - k_begin - warp > 0 ? (k_end - k_begin - warp + WARPS - 1) / WARPS : 0;
+    uint32_t good = 0;  // bit: the step in that stage has a page
+    int issued = 0;
+    auto issue = [&]() {
+      if (issued < my_steps) {
+        if (issued >= ids_at + 32) {
+          ids_at = issued;
+          const int k = k_begin + warp + WARPS * (ids_at + lane);
+          page_ids = k < k_end ? table[k >> 1] : -1;
+        }
+        const int page = __shfl_sync(0xffffffffu, page_ids, issued - ids_at);
+        const int k = k_begin + warp + WARPS * issued;
+        const int stage = issued % C::STAGES;
+        const bool ok = page >= 0 && page < a.pages;
+        good = (good & ~(1u << stage)) | (static_cast<uint32_t>(ok) << stage);
+        if (ok) {
+          const uint8_t* src = a.cache + (static_cast<long long>(page) * a.kv_heads + head) * L::PAGE_BYTES +
+                               (k & 1) * C::STEP_BYTES;
+          const uint32_t dst = ring + stage * C::STEP_BYTES;
+#pragma unroll
+          for (int i = 0; i < (C::STEP_BYTES + 511) / 512; ++i)
+            if (i * 512 + lane * 16 < C::STEP_BYTES) cp_async16(dst + i * 512 + lane * 16, src + i * 512 + lane * 16);
+        }
+        ++issued;
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < C::STAGES - 1; ++i) issue();
+
+    // ---- query rows, 16 bytes per thread and turn, in the order of the B fragments
+    constexpr int PER_ROW = D / 8;
+#pragma unroll
+    for (int i = 0; i < C::ROWS * PER_ROW; i += THREADS) {
+      const int at = i + threadIdx.x;
+      if (C::ROWS * PER_ROW % THREADS == 0 || at < C::ROWS * PER_ROW) {
+        const int row = at / PER_ROW, ch = at % PER_ROW;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (row < nrows) {
+          const int t = (row0 + row) / a.group, g = (row0 + row) % a.group;
+          x = *reinterpret_cast<const uint4*>(a.q + (rows.first + t) * a.q_stride_t +
+                                              (static_cast<long long>(head) * a.group + g) * a.q_stride_h + ch * 8);
+        }
+        float f = 1.f;
+        if (BF16) {
+          // bf16 rows are scaled by a power of two that brings their largest
+          // number to [1, 2) and then fit fp16: what falls below 2^-24 of the
+          // largest is lost, less than the 32-bit sums keep
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          float y[8], mx = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 v = bf162_to_float2(w[e]);
+            y[2 * e] = v.x;
+            y[2 * e + 1] = v.y;
+            mx = fmaxf(mx, fmaxf(fabsf(v.x), fabsf(v.y)));
+          }
+#pragma unroll
+          for (int d = PER_ROW / 2; d > 0; d /= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          const uint32_t ex = (__float_as_uint(mx) >> 23) & 255u;
+          if (ex > 0 && ex < 254) {  // not for zeros, subnormal rows and infinities
+            f = __uint_as_float(ex << 23);
+            const float inv = __uint_as_float((254u - ex) << 23);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] *= inv;
+          }
+          x = make_uint4(fa::pack_half2(y[0], y[1]), fa::pack_half2(y[2], y[3]), fa::pack_half2(y[4], y[5]),
+                         fa::pack_half2(y[6], y[7]));
+        }
+        if (ch == 0) rowf[row] = f;
+        // chunk ch of the row: lane c = ch / (D/32), pair of k-steps ch % (D/32)
+        const int lane_to = (row % 8) * 4 + ch / (D / 32);
+        *reinterpret_cast<uint4*>(smem + C::Q_OFF + (((row / 8) * (D / 32) + ch % (D / 32)) * 32 + lane_to) * 16) = x;
+      }
+    }
+    __syncthreads();
+
+    Acc<D, NT> acc;
+    float factor[NT][2];
+    int limit[NT][2];
+    const float kf = a.scale_log2 * (a.k_scale ? a.k_scale[head] : 1.f);
+    int least = INT_MAX;  // first token that some row of the unit does not see
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = nt * 8 + 2 * c + i;
+        factor[nt][i] = kf * rowf[row];
+        limit[nt][i] = a.causal && row < nrows ? len - rows.n + 1 + (row0 + row) / a.group : len;
+        acc.m[nt][i] = -INFINITY;
+        acc.l[nt][i] = 0.f;
+      }
+    least = a.causal ? min(len, len - rows.n + 1 + row0 / a.group) : len;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc.o[t][nt][e] = 0.f;
+
+    // ---- this warp's steps
+    for (int i = 0; i < my_steps; ++i) {
+      issue();
+      cp_async_wait<C::STAGES - 1>();
+      __syncwarp();
+      const int stage = i % C::STAGES;
+      if ((good >> stage) & 1u) {
+        const int key0 = (k_begin + warp + WARPS * i) * STEP;
+        if (key0 + STEP > least)
+          step<D, NT, true>(acc, ring + stage * C::STEP_BYTES, s0 + C::Q_OFF, lane, factor, key0, len, limit);
+        else
+          step<D, NT, false>(acc, ring + stage * C::STEP_BYTES, s0 + C::Q_OFF, lane, factor, key0, len, limit);
+      }
+      __syncwarp();  // the stage is free for the next copy
+    }
+    cp_async_wait<0>();
+
+    // ---- the four warps' sums become one
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float l = acc.l[nt][i];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        acc.l[nt][i] = l;
+        // a row of NaN scores has no maximum, but its sums are NaN and stay
+        if (acc.m[nt][i] == -INFINITY && l != l) acc.m[nt][i] = 0.f;
+        if (n == 0) ml[warp * C::ROWS + nt * 8 + 2 * c + i] = make_float2(acc.m[nt][i], l);
+      }
+    __syncthreads();
+    float* mine = reinterpret_cast<float*>(smem + warp * C::RING);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = nt * 8 + 2 * c + i;
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, ml[w * C::ROWS + row].x);
+        const float f = acc.m[nt][i] == -INFINITY ? 0.f : fa::ex2_approx(acc.m[nt][i] - m);
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t)
+          *reinterpret_cast<float2*>(mine + row * C::LD + n * (D / 8) + 2 * t) =
+              make_float2(acc.o[t][nt][i] * f, acc.o[t][nt][2 + i] * f);
+      }
+    __syncthreads();
+    const bool starts = off == 0, ends = stop == sh.steps;
+    const long long slot = static_cast<long long>(blockIdx.x) * 2 + (starts ? 1 : 0);
+    const float vf = a.v_scale ? a.v_scale[head] : 1.f;
+    for (int at = threadIdx.x; at < nrows * (D / 4); at += THREADS) {
+      const int row = at / (D / 4), d = at % (D / 4) * 4;
+      float m = -INFINITY, l = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) m = fmaxf(m, ml[w * C::ROWS + row].x);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float2 u = ml[w * C::ROWS + row];
+        l += u.x == -INFINITY ? 0.f : u.y * fa::ex2_approx(u.x - m);
+        const float4 y = *reinterpret_cast<const float4*>(smem + w * C::RING + (row * C::LD + d) * 4);
+        x.x += y.x;
+        x.y += y.y;
+        x.z += y.z;
+        x.w += y.w;
+      }
+      if (starts && ends) {
+        const float inv = m == -INFINITY ? 0.f : vf / l;
+        const int t = (row0 + row) / a.group, g = (row0 + row) % a.group;
+        store4<BF16>(a.o + (rows.first + t) * a.o_stride_t +
+                         (static_cast<long long>(head) * a.group + g) * a.o_stride_h + d,
+                     make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+      } else {
+        *reinterpret_cast<float4*>(p.part_o + (slot * C::ROWS + row) * D + d) = x;
+        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * C::ROWS + row) * 2) = make_float2(m, l);
+      }
+    }
+    if (starts && !ends) {
+      const int last = range_owner(pos - off + sh.steps - 1, total, blocks);
+      rec = {last - static_cast<int>(blockIdx.x) + 1, rows.first, row0, nrows, head, {0, 0, 0}};
+    }
+    pos += stop - off;
+    __syncthreads();  // the merge buffers, Q and row factors are free
+  }
+  if (threadIdx.x == 0) p.record[blockIdx.x] = rec;
+}
+
+// Joins the pieces of the unit that block blockIdx.x started and did not end:
+// its own second slot and the first slots of the blocks after it, in that
+// order. Also zeroes the rows behind the last request, when asked to.
+template <int D, int NT, bool BF16>
+__global__ void __launch_bounds__(256) cache4_join_kernel(const FewParams p) {
+  constexpr int ROWS = 8 * NT;
+  constexpr int V = D / 32;  // channels of a lane
+  __shared__ float red[8][D + 2];
+  const AttnParams& a = p.a;
+  fa::griddep_wait();
+  if (threadIdx.x == 0) fa::griddep_launch_dependents();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (a.zero_rest) {
+    const int from = min(max(a.query_start[a.requests], 0), a.tokens);
+    const long long per = static_cast<long long>(a.kv_heads) * a.group * (D / 4);
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < (a.tokens - from) * per; i += gridDim.x * 256ll) {
+      const long long t = from + i / per, h = i % per / (D / 4);
+      store4<BF16>(a.o + t * a.o_stride_t + h * a.o_stride_h + i % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+    }
+  }
+  const JoinRecord rec = p.record[blockIdx.x];
+  if (rec.pieces == 0) return;
+  // 8 warps: `parts` of them share a row's pieces
+  const int parts = rec.rows <= 1 ? 8 : rec.rows <= 2 ? 4 : rec.rows <= 4 ? 2 : 1;
+  const int part = warp % parts;
+  const float vf = a.v_scale ? a.v_scale[rec.head] : 1.f;
+  for (int row = warp / parts; row < (rec.rows + 8 / parts - 1) / (8 / parts) * (8 / parts); row += 8 / parts) {
+    const bool there = row < rec.rows;
+    auto slot_row = [&](int k) -> long long {
+      const long long slot = k == 0 ? blockIdx.x * 2ll + 1 : (static_cast<long long>(blockIdx.x) + k) * 2;
+      return slot * ROWS + row;
+    };
+    float m = -INFINITY, l = 0.f, x[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = 0.f;
+    if (there) {
+      for (int k = lane; k < rec.pieces; k += 32) m = fmaxf(m, p.part_ml[slot_row(k) * 2]);
+#pragma unroll
+      for (int d = 16; d > 0; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      if (m > -INFINITY) {
+#pragma unroll 4
+        for (int k = part; k < rec.pieces; k += parts) {
+          const long long at = slot_row(k);
+          const float2 u = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+          const float f = u.x == -INFINITY ? 0.f : fa::ex2_approx(u.x - m);
+          l += u.y * f;
+          if (V == 4) {
+            const float4 y = *reinterpret_cast<const float4*>(p.part_o + at * D + lane * V);
+            x[0] += y.x * f;
+            x[1] += y.y * f;
+            x[V - 2] += y.z * f;
+            x[V - 1] += y.w * f;
+          } else {
+            const float2 y = *reinterpret_cast<const float2*>(p.part_o + at * D + lane * V);
+            x[0] += y.x * f;
+            x[1] += y.y * f;
+          }
+        }
+      }
+    }
+    if (parts > 1) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) red[warp][lane * V + e] = x[e];
+      if (lane == 0) red[warp][D] = l;
+      __syncthreads();
+      if (part == 0) {
+        for (int k = 1; k < parts; ++k) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) x[e] += red[warp + k][lane * V + e];
+          l += red[warp + k][D];
+        }
+      }
+      __syncthreads();
+    }
+    if (there && part == 0) {
+      const float inv = m == -INFINITY ? 0.f : vf / l;
+      const int t = (rec.row0 + row) / a.group, g = (rec.row0 + row) % a.group;
+      uint16_t* dst = a.o + (rec.first + t) * a.o_stride_t +
+                      (static_cast<long long>(rec.head) * a.group + g) * a.o_stride_h + lane * V;
+#pragma unroll
+      for (int e = 0; e < V; e += 2)
+        *reinterpret_cast<uint32_t*>(dst + e) = float2_to_pair<BF16>(x[e] * inv, x[e + 1] * inv);
+    }
+  }
+}
+
+// -------------------------------------------------------------------- host
+static bool args_ok(const gfx906_b200_cache4_attn_args& g) {
+  return g.dtype >= 0 && g.dtype <= 1 && g.tokens >= 0 && g.heads > 0 && g.kv_heads > 0 && g.heads % g.kv_heads == 0 &&
+         g.pages >= 0 && g.requests >= 0 && g.requests <= MAX_CHUNKS * THREADS && g.width >= 0 &&
+         g.width <= INT_MAX / PAGE && g.max_tokens >= 0 && isfinite(g.scale) &&
+         static_cast<long long>(g.tokens) * (g.heads / g.kv_heads) <= INT_MAX;
+}
+
+struct Plan {
+  int nt;      // row tiles of 8 NT rows
+  int blocks;
+  size_t ml_off, rec_off, bytes;
+};
+static Plan plan_of(const gfx906_b200_cache4_attn_args& g, int sms) {
+  Plan pl{};
+  const long long rows = static_cast<long long>(g.max_tokens) * (g.heads / g.kv_heads);
+  pl.nt = rows <= 8 ? 1 : 2;
+  pl.blocks = sms * (pl.nt == 1 ? 4 : 3);
+  const size_t slots = static_cast<size_t>(pl.blocks) * 2 * 8 * pl.nt;
+  pl.ml_off = slots * g.D * sizeof(float);
+  pl.rec_off = pl.ml_off + slots * 2 * sizeof(float);
+  pl.bytes = (pl.rec_off + pl.blocks * sizeof(JoinRecord) + 255) & ~static_cast<size_t>(255);
+  return pl;
+}
+
+template <int D, int NT, bool BF16>
+static int launch_few(const FewParams& p, int blocks, cudaStream_t stream) {
+  const cudaError_t e = cudaFuncSetAttribute(cache4_few_kernel<D, NT, BF16>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, Few<D, NT>::SMEM);
+  if (e != cudaSuccess) return GFX906_B200_ECUDA;
+  const int rc = launch(cache4_few_kernel<D, NT, BF16>, dim3(blocks), dim3(THREADS), Few<D, NT>::SMEM, stream, p);
+  if (rc != GFX906_B200_OK) return rc;
+  return launch(cache4_join_kernel<D, NT, BF16>, dim3(blocks), dim3(256), 0, stream, p);
+}
+template <int D, int NT>
+static int launch_few_t(const FewParams& p, int dtype, int blocks, cudaStream_t stream) {
+  return dtype ? launch_few<D, NT, true>(p, blocks, stream) : launch_few<D, NT, false>(p, blocks, stream);
+}
+
+static int attn(const gfx906_b200_cache4_attn_args& g, void* ws, size_t ws_bytes, cudaStream_t stream) {
+  if (!head_dim_ok(g.D)) return GFX906_B200_EHEADDIM;
+  if (!args_ok(g)) return GFX906_B200_EINVAL;
+  if (g.tokens == 0) return GFX906_B200_OK;
+  if (!g.q || !g.o || !g.query_start || (g.requests && !g.lengths) || (g.pages && !g.cache) ||
+      (static_cast<long long>(g.requests) * g.width && !g.tables))
+    return GFX906_B200_EINVAL;
+  if (!aligned16(g.q) || !aligned16(g.o) || !aligned16(g.cache) ||
+      ((g.q_stride_t | g.q_stride_h | g.o_stride_t | g.o_stride_h) & 7))
+    return GFX906_B200_EALIGN;
+  int sms = 0;
+  const int rc = gfx906_b200_internal_device(&sms);
+  if (rc != GFX906_B200_OK) return rc;
+  const Plan pl = plan_of(g, sms);
+  if (!ws || ws_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(ws) & 255u)) return GFX906_B200_EINVAL;
+  FewParams p{};
+  p.a = {static_cast<const uint16_t*>(g.q), static_cast<uint16_t*>(g.o), static_cast<const uint8_t*>(g.cache), g.tables,
+         g.lengths, g.query_start, g.k_scale, g.v_scale, g.q_stride_t, g.q_stride_h, g.o_stride_t, g.o_stride_h,
+         g.tokens, g.kv_heads, g.heads / g.kv_heads, g.pages, g.requests, g.width, g.causal != 0, g.zero_rest != 0,
+         g.scale * 1.4426950408889634f};
+  p.max_rows = INT_MAX;
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  p.part_o = reinterpret_cast<float*>(base);
+  p.part_ml = reinterpret_cast<float*>(base + pl.ml_off);
+  p.record = reinterpret_cast<JoinRecord*>(base + pl.rec_off);
+  if (g.D == 128)
+    return pl.nt == 1 ? launch_few_t<128, 1>(p, g.dtype, pl.blocks, stream)
+                      : launch_few_t<128, 2>(p, g.dtype, pl.blocks, stream);
+  return pl.nt == 1 ? launch_few_t<64, 1>(p, g.dtype, pl.blocks, stream)
+                    : launch_few_t<64, 2>(p, g.dtype, pl.blocks, stream);
+}
+
+}  // namespace c4
+
+extern "C" {
+
+size_t gfx906_b200_cache4_attn_workspace_size(const gfx906_b200_cache4_attn_args* args) {
+  int sms = 0;
+  if (!args || !c4::head_dim_ok(args->D) || !c4::args_ok(*args) || args->tokens == 0 ||
+      gfx906_b200_internal_device(&sms) != GFX906_B200_OK)
+    return 0;
+  return c4::plan_of(*args, sms).bytes;
+}
+
+int gfx906_b200_cache4_attn(const gfx906_b200_cache4_attn_args* args, void* workspace, size_t workspace_bytes,
+                            cudaStream_t stream) {
+  if (!args) return c4::done(GFX906_B200_EINVAL);
+  return c4::done(c4::attn(*args, workspace, workspace_bytes, stream));
+}
+
+}  // extern "C"

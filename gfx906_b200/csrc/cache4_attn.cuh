@@ -1,0 +1,38 @@
+// Parameters shared by the attention kernels over the 4-bit cache.
+#pragma once
+
+#include <stdint.h>
+
+namespace c4 {
+
+struct AttnParams {
+  const uint16_t* q;  // fp16 or bf16
+  uint16_t* o;
+  const uint8_t* cache;
+  const int* tables;
+  const int* lengths;
+  const int* query_start;
+  const float* k_scale;
+  const float* v_scale;
+  long long q_stride_t, q_stride_h, o_stride_t, o_stride_h;
+  int tokens, kv_heads, group, pages, requests, width;
+  int causal, zero_rest;
+  float scale_log2;  // scale * log2(e)
+};
+
+// Query rows of request r: first token and number of tokens, whatever the
+// array holds (it comes from the caller's device memory).
+struct Rows {
+  int first, n;
+};
+__device__ __forceinline__ Rows rows_of(const AttnParams& p, int r) {
+  const int a = min(max(p.query_start[r], 0), p.tokens), b = min(max(p.query_start[r + 1], 0), p.tokens);
+  return {a, max(b - a, 0)};
+}
+__device__ __forceinline__ int length_of(const AttnParams& p, int r) {
+  const long long most = static_cast<long long>(p.width) * 64;
+  const int n = max(p.lengths[r], 0);
+  return n < most ? n : static_cast<int>(most);
+}
+
+}  // namespace c4
