@@ -38,8 +38,9 @@ EXT_PATH = PKG_DIR / (EXT_NAME + (sysconfig.get_config_var("EXT_SUFFIX") or ".so
 
 # Every CUDA translation unit of the library.
 CU_SOURCES = [CSRC / "attn_fwd_sm100.cu", CSRC / "attn_fwd_noalloc.cu", CSRC / "cache4_store.cu",
-              CSRC / "cache4_attn.cu"]
-CU_HEADERS = [CSRC / "sm100_ptx.cuh", CSRC / "cache4.cuh", CSRC / "cache4_attn.cuh", CSRC / "cache4_host.cuh",
+              CSRC / "cache4_attn.cu", CSRC / "cache4_many.cu"]
+CU_HEADERS = [CSRC / "sm100_ptx.cuh", CSRC / "attn_row.cuh", CSRC / "cache4.cuh", CSRC / "cache4_attn.cuh",
+              CSRC / "cache4_many.cuh", CSRC / "cache4_host.cuh",
               INCLUDE / "gfx906_b200_attn.h", INCLUDE / "gfx906_b200_cache4.h"]
 # The torch operator module and the headers it shares with the library.
 EXT_SOURCES = [CSRC / "attn.cpp", CSRC / "cache4.cpp"]

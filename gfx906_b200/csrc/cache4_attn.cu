@@ -25,9 +25,14 @@
 #include "cache4.cuh"
 #include "cache4_attn.cuh"
 #include "cache4_host.cuh"
+#include "cache4_many.cuh"
 #include "sm100_ptx.cuh"
 
 namespace c4 {
+
+// Requests with more query rows (tokens times heads of a group) go to the
+// tensor-memory kernel of cache4_many.cu.
+constexpr int FEW_ROWS = 64;
 
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
@@ -665,7 +670,8 @@ static bool args_ok(const gfx906_b200_cache4_attn_args& g) {
 struct Plan {
   int nt;      // row tiles of 8 NT rows
   int blocks;
-  size_t ml_off, rec_off, bytes;
+  size_t ml_off, rec_off, many_off, bytes;
+  ManyPlan many;  // max_blocks 0: no request has that many rows
 };
 static Plan plan_of(const gfx906_b200_cache4_attn_args& g, int sms) {
   Plan pl{};
@@ -675,7 +681,9 @@ static Plan plan_of(const gfx906_b200_cache4_attn_args& g, int sms) {
   const size_t slots = static_cast<size_t>(pl.blocks) * 2 * 8 * pl.nt;
   pl.ml_off = slots * g.D * sizeof(float);
   pl.rec_off = pl.ml_off + slots * 2 * sizeof(float);
-  pl.bytes = (pl.rec_off + pl.blocks * sizeof(JoinRecord) + 255) & ~static_cast<size_t>(255);
+  pl.many_off = (pl.rec_off + pl.blocks * sizeof(JoinRecord) + 255) & ~static_cast<size_t>(255);
+  if (rows > FEW_ROWS) pl.many = many_plan(g.tokens, g.requests, g.heads / g.kv_heads, g.kv_heads, g.D, sms);
+  pl.bytes = pl.many_off + ((pl.many.bytes + 255) & ~static_cast<size_t>(255));
   return pl;
 }
 
@@ -715,6 +723,18 @@ static int attn(const gfx906_b200_cache4_attn_args& g, void* ws, size_t ws_bytes
          g.scale * 1.4426950408889634f};
   p.max_rows = INT_MAX;
   uint8_t* base = static_cast<uint8_t*>(ws);
+  if (pl.many.max_blocks > 0) {
+    ManyParams m{};
+    m.a = p.a;
+    m.min_rows = p.max_rows = FEW_ROWS;
+    m.max_blocks = pl.many.max_blocks;
+    m.pieces = pl.many.pieces;
+    m.part_o = reinterpret_cast<float*>(base + pl.many_off);
+    m.part_ml = reinterpret_cast<float*>(base + pl.many_off + pl.many.ml_off);
+    m.timeout_ns = gfx906_b200_internal_timeout_ns();
+    const int st = launch_many(m, g.D, g.dtype, stream);
+    if (st != GFX906_B200_OK) return st;
+  }
   p.part_o = reinterpret_cast<float*>(base);
   p.part_ml = reinterpret_cast<float*>(base + pl.ml_off);
   p.record = reinterpret_cast<JoinRecord*>(base + pl.rec_off);

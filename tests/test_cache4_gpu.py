@@ -290,6 +290,67 @@ def test_attention_few_tokens(shape, D, dtype):
     p.check(p.run(max_tokens=most, causal=False), causal=False)
 
 
+MANY = [  # counts, lengths, kv heads, group, rows checked
+    ([65], [65], 1, 1, range(65)), ([130], [130], 1, 1, range(130)), ([100], [77], 1, 2, range(100)),
+    ([257], [300], 2, 1, [0, 1, 43, 84, 85, 127, 128, 129, 213, 255, 256]),
+    ([33], [1000], 1, 4, range(33)), ([129, 40], [129, 2000], 2, 3, [0, 1, 39, 40, 63, 64, 85, 86, 127, 128]),
+    ([1, 90, 0, 3, 64, 300, 2], [700, 90, 5, 1, 64, 513, 130], 1, 2, [0, 1, 2, 63, 64, 89, 127, 128, 255, 256, 299]),
+    ([600], [4500], 1, 1, [0, 127, 128, 255, 256, 511, 512, 599]),
+    ([70] * 30, [(61 * i) % 300 + 70 for i in range(30)], 5, 1, [0, 63, 69]),  # enough units for every SM
+]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", MANY, ids=range(len(MANY)))
+def test_attention_many_tokens(shape, D, dtype):
+    p = Problem(*shape[:4], D, dtype, seed=len(shape[0]))
+    p.check(p.run(), rows=shape[4])
+    p.check(p.run(causal=False), causal=False, rows=shape[4])
+    assert torch.equal(p.run(), p.run())
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1.5])
+def test_attention_many_tokens_scales(scale):
+    p = Problem([150], [400], 1, 1, 64, torch.float16)
+    p.check(p.run(scale=scale), scale=scale, rows=[0, 77, 149])
+
+
+def test_attention_many_tokens_bad_pages_nan_queries_and_strides():
+    p = Problem([140, 200], [300, 500], 2, 1, 128, torch.float16)
+    p.tables[0][0] = -1
+    p.tables[0][3] = 10 ** 9
+    p.tables[1][2] = 10 ** 9
+    p.q[7, 1] = float("nan")
+    q = torch.zeros(340, 5, 128, dtype=torch.float16, device="cuda")
+    q[:, 2:4] = p.q.cuda()
+    out = p.run(q=q[:, 2:4], causal=False)
+    assert out[7, 1].isnan().all()
+    p.q[7, 1] = 0
+    out[7, 1] = p.run(causal=False)[7, 1]
+    for r, gone in ((0, [0, 3]), (1, [2])):
+        keep = [i for i in range(p.lengths[r]) if i // 64 not in gone]
+        p.k[r], p.v[r], p.lengths[r] = p.k[r][keep], p.v[r][keep], len(keep)
+    p.check(out, causal=False, rows=[0, 7, 8, 127, 128, 139, 199])
+
+
+def test_attention_many_tokens_growing_scores():
+    """Scores that grow along the keys move every row's maximum again and again."""
+    p = Problem([130], [700], 1, 1, 64, torch.float16)
+    p.q *= torch.linspace(0.0, 6.0, 130)[:, None, None].half()
+    p.q += 0.5
+    p.k[0] += 0.02 * torch.arange(700)[:, None, None]
+    slots = ints([p.tables[0][i // 64] * 64 + i % 64 for i in range(700)])
+    g.cache4_write(p.k[0].half().cuda(), p.v[0].half().cuda(), p.cache, slots, *p.factors())
+    k, v = g.cache4_read(p.cache, slots, *p.factors(), dtype=torch.float32)
+    p.k[0], p.v[0] = k.cpu(), v.cpu()
+    out = p.run(causal=False).cpu()
+    for i in (0, 1, 60, 129):
+        ref, size = oracle.attention(p.q[i], p.k[0][:, 0], p.v[0][:, 0], p.scale, False)
+        # scores up to 600: 32 bits hold them to 600 * 2^-24 * 64 products, far less than 2^-8 of p
+        assert ((out[i, 0].double() - ref[0]).abs() <= size[0] * 2.0 ** -8 + 2.0 ** -11 * ref[0].abs() + 1e-4).all(), i
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_attention_long_context_is_split(D):
     p = Problem([1, 1], [20011, 37], 2, 4, D, torch.float16, factors=False)
