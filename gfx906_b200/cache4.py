@@ -59,10 +59,17 @@ class Cache4Plan(NamedTuple):
     free_count: torch.Tensor   # [1] free pages left
 
 
-def _module():
-    from . import _module_or_raise
+_loaded = None
 
-    return _module_or_raise()
+
+def _module():
+    """The operator module, or RuntimeError; kept, as these calls are as short as the look-up."""
+    global _loaded
+    if _loaded is None:
+        from . import _module_or_raise
+
+        _loaded = _module_or_raise()
+    return _loaded
 
 
 def cache4_alloc(pages, kv_heads, head_dim, device="cuda"):

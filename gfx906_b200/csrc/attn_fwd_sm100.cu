@@ -2068,6 +2068,7 @@ int gfx906_b200_internal_device(int* num_sms) {
 }
 
 unsigned long long gfx906_b200_internal_timeout_ns(void) { return timeout_ns_from_env(); }
+unsigned long long gfx906_b200_internal_next_epoch(void) { return next_epoch(); }
 
 int gfx906_b200_attn_launch_ws(const void* q, const void* k, const void* v, void* o, int B, int H, int Sq,
                                int Skv, int D, float scale, void* workspace, size_t workspace_bytes,

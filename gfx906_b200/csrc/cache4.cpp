@@ -81,14 +81,15 @@ PlanOut cache4_plan(Tensor tables, Tensor lengths, Tensor counts, Tensor free_pa
   TORCH_CHECK(W <= INT32_MAX / kPage && R * W <= INT32_MAX && free_pages.size(0) <= INT32_MAX, "cache4: sizes are too large");
   TORCH_CHECK(tokens >= 0 && tokens < INT32_MAX, "cache4: tokens must be a non-negative int32");
   const c10::cuda::CUDAGuard guard(tables.device());
-  auto like = tables.options();
-  // one allocation, cut at 16 bytes: a decoding step is launch-bound
-  auto up = [](int64_t n) { return (n + 3) / 4 * 4; };
-  Tensor all = torch::empty({up(R + 1) + 2 * up(R) + 2 * up(tokens) + 1}, like);
+  // One allocation cut into the six results: a decoding step is bound by its launches.
+  const Tensor all = torch::empty({3 * R + 2 * tokens + 2}, tables.options());
   int64_t at = 0;
   auto cut = [&](int64_t n) {
-    Tensor t = all.narrow(0, at, n);
-    at += up(n);
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(all.storage()),
+                                                        all.key_set(), all.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(at);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    at += n;
     return t;
   };
   Tensor query_start = cut(R + 1), lengths_out = cut(R), added = cut(R), slots = cut(tokens), positions = cut(tokens),

@@ -8,7 +8,7 @@
 // copy of 36 D bytes). The steps of all units form one line that the blocks
 // share evenly, whatever the requests' lengths; a unit that is cut at a block's
 // end leaves partial sums (m, l, unnormalised O, 32 bits) in the workspace,
-// joined by cache4_join_kernel. Every unit counts one step more than it has
+// joined by the block that finishes its last piece. Every unit counts one step more than it has
 // keys for, so that units without any key have an owner that writes their
 // zeros, and as the price of starting a unit.
 //
@@ -34,33 +34,37 @@ namespace c4 {
 // tensor-memory kernel of cache4_many.cu.
 constexpr int FEW_ROWS = 64;
 
-constexpr int WARPS = 4;
-constexpr int THREADS = WARPS * 32;
+#ifndef FEW_WARPS
+#define FEW_WARPS 4
+#endif
+#ifndef FEW_MIN
+#define FEW_MIN 1
+#endif
+constexpr int MAX_REQUESTS = 8192;
 constexpr int STEP = 32;                // tokens of a step
-constexpr int MAX_CHUNKS = 64;          // of THREADS requests
-constexpr int MIN_STEPS = WARPS;        // fewest steps a block is started for
-constexpr int RECORD_INTS = 8;
-
-struct JoinRecord {  // written by the block that starts a cut unit
-  int pieces;        // 0: nothing to join
-  int first;         // first token of the request
-  int row0, rows;    // query rows of the unit
-  int head;          // kv head
-  int pad[3];
-};
-static_assert(sizeof(JoinRecord) == RECORD_INTS * 4, "");
+constexpr float REACH = 8.f;            // see step()
 
 struct FewParams {
   AttnParams a;
   int max_rows;       // requests with more query rows are another kernel's
   float* part_o;      // [blocks][2][8 NT][D]
   float* part_ml;     // [blocks][2][8 NT][2]
-  JoinRecord* record; // [blocks]
+  // [blocks] pieces in the workspace of the cut unit that the block starts,
+  // tagged with the launch: (epoch << 16) | pieces. Whoever comes first to a
+  // word with another tag sets it to none, so the workspace needs no clearing;
+  // whoever joins a unit sets its word to none again, for a replay of the launch.
+  unsigned long long* done;
+  unsigned long long epoch;
 };
 
 template <int D, int NT>
 struct Few {
   using L = Layout<D>;
+  static constexpr int WARPS = NT == 1 || FEW_WARPS == 4 ? FEW_WARPS : FEW_WARPS == 8 ? 6 : 12;
+  static constexpr int THREADS = WARPS * 32;
+  static constexpr int PER_SM = (NT == 1 ? 16 : 12) / WARPS;  // blocks that share an SM
+  static constexpr int MAX_CHUNKS = (MAX_REQUESTS + THREADS - 1) / THREADS;
+  static constexpr int MIN_STEPS = WARPS * FEW_MIN;  // steps of a unit that are worth a block of their own
   static constexpr int ROWS = 8 * NT;
   static constexpr int STEP_BYTES = 2 * L::BLOCK_BYTES;
   static constexpr int STAGES = NT == 1 ? 2 : 3;  // four or three blocks share an SM
@@ -71,7 +75,7 @@ struct Few {
   static constexpr int ML_OFF = Q_OFF + Q_BYTES;          // [WARPS][ROWS] (m, l)
   static constexpr int ROWF_OFF = ML_OFF + WARPS * ROWS * 8;  // [ROWS] factors of the rows of q
   static constexpr int SMEM = ROWF_OFF + ROWS * 4;
-  static_assert(ROWS * LD * 4 <= RING, "a warp's merge buffer is its ring");
+  static_assert(PER_SM >= 1 && ROWS * LD * 4 <= RING, "a warp's merge buffer is its ring");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -82,31 +86,17 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t lds16(uint32_t a) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
-  return v;
-}
 // W words at a, W = 2 or 4.
 template <int W>
-__device__ __forceinline__ void lds(uint32_t a, uint32_t* v) {
+__device__ __forceinline__ void lds(const uint8_t* a, uint32_t* v) {
   if (W == 4)
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                 : "r"(a)
-                 : "memory");
+    *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(a);
   else
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a) : "memory");
+    *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(a);
 }
 __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -117,18 +107,17 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return r;
 }
 
-// Steps (plus one) and units of a request; 0 units when it is not ours.
+// One request's part of the line of steps.
 struct Share {
-  long long weight;  // of the whole request
-  int steps;         // of one unit, with the one extra
+  int first, rows, len;  // first token; query rows (0: not this kernel's); keys
+  int units, steps;      // units; steps of one unit, with the one extra
 };
 template <int ROWS>
 __device__ __forceinline__ Share share_of(const FewParams& p, int r) {
-  const int n = rows_of(p.a, r).n;
-  const long long rows = static_cast<long long>(n) * p.a.group;
-  if (n == 0 || rows > p.max_rows) return {0, 0};
-  const int steps = (length_of(p.a, r) + STEP - 1) / STEP + 1;
-  return {(rows + ROWS - 1) / ROWS * p.a.kv_heads * steps, steps};
+  const Rows t = rows_of(p.a, r);
+  const int len = length_of(p.a, r), rows = t.n * p.a.group;
+  if (rows > p.max_rows) return {t.first, 0, len, 0, 0};
+  return {t.first, rows, len, (rows + ROWS - 1) / ROWS * p.a.kv_heads, rows ? (len + STEP - 1) / STEP + 1 : 0};
 }
 
 // Per-thread state of one warp's share of a unit.
@@ -142,9 +131,14 @@ struct Acc {
 // MASK: tokens key0 + 0..31 may lie behind the last one a row sees
 // (limit[nt][i], exclusive) or behind the request's length (`len`): those keys
 // take no part, and their values -- whatever the page holds there -- are zeroed.
+//
+// A row's m is a reference that its scores may exceed by REACH (log2 units), not
+// their maximum: P then stays below 2^REACH, O and l carry the same factor, and
+// the maximum across the warp, with the products that follow from it, is taken
+// only in the few steps where a vote finds a score beyond reach.
 template <int D, int NT, bool MASK>
-__device__ __forceinline__ void step(Acc<D, NT>& acc, uint32_t blk, uint32_t sq, int lane, const float (&factor)[NT][2],
-                                     int key0, int len, const int (&limit)[NT][2]) {
+__device__ __forceinline__ void step(Acc<D, NT>& acc, const uint8_t* blk, const uint8_t* sq, int lane,
+                                     const float (&factor)[NT][2], int key0, int len, const int (&limit)[NT][2]) {
   using L = Layout<D>;
   constexpr int W = D / 32;  // words of K codes of a lane and token
   const int n = lane >> 2, c = lane & 3;
@@ -156,109 +150,118 @@ __device__ __forceinline__ void step(Acc<D, NT>& acc, uint32_t blk, uint32_t sq,
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[b][nt][e] = 0.f;
   // ---- S^T = K Q^T
+  {
+    uint32_t k[2][2][W];        // block, tokens n and n + 8
+    uint32_t f[2][2][L::GPL];   // their scales, in both halves
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    const uint32_t base = blk + b * L::BLOCK_BYTES;
-    uint32_t k0[W], k1[W];  // tokens n and n + 8
-    lds<W>(base + L::KC + lane * (D / 8), k0);
-    lds<W>(base + L::KC + 4 * D + lane * (D / 8), k1);
-    uint32_t f0[L::GPL], f1[L::GPL];  // scales of tokens n and n + 8, in both halves
-    if (L::GPL == 2) {
-      const uint32_t w = lds32(base + L::KS + lane * 4);
-      const uint32_t x = scales_to_half2(w), y = scales_to_half2(w >> 16);
-      f0[0] = __byte_perm(x, x, 0x1010);
-      f0[L::GPL - 1] = __byte_perm(x, x, 0x3232);
-      f1[0] = __byte_perm(y, y, 0x1010);
-      f1[L::GPL - 1] = __byte_perm(y, y, 0x3232);
-    } else {
-      const uint32_t x = scales_to_half2(lds16(base + L::KS + lane * 2));
-      f0[0] = __byte_perm(x, x, 0x1010);
-      f1[0] = __byte_perm(x, x, 0x3232);
+    for (int b = 0; b < 2; ++b) {
+      const uint8_t* base = blk + b * L::BLOCK_BYTES;
+      lds<W>(base + L::KC + lane * (D / 8), k[b][0]);
+      lds<W>(base + L::KC + 4 * D + lane * (D / 8), k[b][1]);
+      if (L::GPL == 2) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(base + L::KS + lane * 4);
+        const uint32_t x = scales_to_half2(w), y = scales_to_half2(w >> 16);
+        f[b][0][0] = __byte_perm(x, x, 0x1010);
+        f[b][0][L::GPL - 1] = __byte_perm(x, x, 0x3232);
+        f[b][1][0] = __byte_perm(y, y, 0x1010);
+        f[b][1][L::GPL - 1] = __byte_perm(y, y, 0x3232);
+      } else {
+        const uint32_t x = scales_to_half2(*reinterpret_cast<const uint16_t*>(base + L::KS + lane * 2));
+        f[b][0][0] = __byte_perm(x, x, 0x1010);
+        f[b][1][0] = __byte_perm(x, x, 0x3232);
+      }
     }
 #pragma unroll
     for (int j = 0; j < W; ++j) {  // two k-steps of 16 channels for each word
-      uint32_t x0[4], x1[4];
-      codes_to_half2(k0[j], x0);
-      codes_to_half2(k1[j], x1);
-      const int g = j * 8 / 16;
+      uint32_t q[NT][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x0[e] = mul_half2(x0[e], f0[g]);
-        x1[e] = mul_half2(x1[e], f1[g]);
-      }
+      for (int nt = 0; nt < NT; ++nt) lds<4>(sq + ((nt * W + j) * 32 + lane) * 16, q[nt]);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        uint32_t qf[4];
-        lds<4>(sq + ((nt * W + j) * 32 + lane) * 16, qf);
-        mma16816(s[b][nt], x0[0], x1[0], x0[1], x1[1], qf[0], qf[1]);
-        mma16816(s[b][nt], x0[2], x1[2], x0[3], x1[3], qf[2], qf[3]);
+      for (int b = 0; b < 2; ++b) {
+        uint32_t x0[4], x1[4];
+        codes_to_half2(k[b][0][j], x0);
+        codes_to_half2(k[b][1][j], x1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x0[e] = mul_half2(x0[e], f[b][0][j / 2]);
+          x1[e] = mul_half2(x1[e], f[b][1][j / 2]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816(s[b][nt], x0[0], x1[0], x0[1], x1[1], q[nt][0], q[nt][1]);
+          mma16816(s[b][nt], x0[2], x1[2], x0[3], x1[3], q[nt][2], q[nt][3]);
+        }
       }
     }
   }
   // ---- running softmax; s[b][nt]: tokens 16 b + n (+ 8), rows 2c, 2c + 1
-  uint32_t pb[2][NT][2];
-  float alpha[NT][2];
-  bool grew = false;
+  auto hidden = [&](int b, int nt, int e) { return MASK && key0 + 16 * b + 8 * (e >> 1) + n >= limit[nt][e & 1]; };
+  float y[2][NT][4];
+  float far = -INFINITY;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+  for (int b = 0; b < 2; ++b)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float mx = -INFINITY;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int e = 0; e < 4; ++e) {
+        y[b][nt][e] = hidden(b, nt, e) ? -INFINITY : fmaf(s[b][nt][e], factor[nt][e & 1], -acc.m[nt][e & 1]);
+        far = fmaxf(far, y[b][nt][e]);
+      }
+  if (__any_sync(0xffffffffu, far > REACH)) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x = s[b][nt][2 * e + i] * factor[nt][i];
-          if (MASK && key0 + 16 * b + 8 * e + n >= limit[nt][i]) x = -INFINITY;
-          s[b][nt][2 * e + i] = x;
-          mx = fmaxf(mx, x);
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = i; e < 4; e += 2)
+            if (!hidden(b, nt, e)) mx = fmaxf(mx, __fmul_rn(s[b][nt][e], factor[nt][i]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        if (mx > acc.m[nt][i]) {
+          const float alpha = fa::ex2_approx(acc.m[nt][i] - mx);
+          acc.m[nt][i] = mx;
+          acc.l[nt][i] *= alpha;
+#pragma unroll
+          for (int t = 0; t < D / 16; ++t) {
+            acc.o[t][nt][i] *= alpha;
+            acc.o[t][nt][2 + i] *= alpha;
+          }
         }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-      const float m_new = fmaxf(acc.m[nt][i], mx);
-      grew |= m_new > acc.m[nt][i];
-      alpha[nt][i] = m_new > acc.m[nt][i] ? fa::ex2_approx(acc.m[nt][i] - m_new) : 1.f;
-      acc.m[nt][i] = m_new;
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;  // no key seen yet
-      float sum = 0.f;
+        // rounded as m was, so that the largest score comes to exactly 0, however large
+        const float m_use = acc.m[nt][i] == -INFINITY ? 0.f : acc.m[nt][i];
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float x = fa::ex2_approx(s[b][nt][2 * e + i] - m_use);
-          s[b][nt][2 * e + i] = x;
-          sum += x;
-        }
-      acc.l[nt][i] = acc.l[nt][i] * alpha[nt][i] + sum;
-    }
-    // P in fp16 (it is at most 1; the sum keeps 32 bits), transposed into B fragments
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        pb[b][nt][e] = transpose8x8(fa::pack_half2(s[b][nt][2 * e], s[b][nt][2 * e + 1]));
-  }
-  if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-    for (int t = 0; t < D / 16; ++t)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        acc.o[t][nt][0] *= alpha[nt][0];
-        acc.o[t][nt][1] *= alpha[nt][1];
-        acc.o[t][nt][2] *= alpha[nt][0];
-        acc.o[t][nt][3] *= alpha[nt][1];
+          for (int e = i; e < 4; e += 2)
+            y[b][nt][e] = hidden(b, nt, e) ? -INFINITY : __fsub_rn(__fmul_rn(s[b][nt][e], factor[nt][i]), m_use);
       }
   }
+  // P in fp16 (the sum keeps 32 bits), transposed into B fragments
+  uint32_t pb[2][NT][2];
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float p0 = fa::ex2_approx(y[b][nt][2 * h]), p1 = fa::ex2_approx(y[b][nt][2 * h + 1]);
+        acc.l[nt][0] += p0;
+        acc.l[nt][1] += p1;
+        pb[b][nt][h] = transpose8x8(fa::pack_half2(p0, p1));
+      }
   // ---- O^T += V^T P^T
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
-    const uint32_t base = blk + b * L::BLOCK_BYTES;
+    const uint8_t* base = blk + b * L::BLOCK_BYTES;
     constexpr int W2 = D / 64;      // words of V codes of a lane and token
     uint32_t v0[2 * W2], v1[2 * W2];  // tokens 2c, 2c + 1; tokens 2c + 8, 2c + 9
     lds<2 * W2>(base + L::VC + lane * (D / 8), v0);
     lds<2 * W2>(base + L::VC + 4 * D + lane * (D / 8), v1);
-    uint32_t w = lds32(base + L::VS + (D == 128 ? lane : (n / 2) * 4 + c) * 4);
+    uint32_t w = *reinterpret_cast<const uint32_t*>(base + L::VS + (D == 128 ? lane : (n / 2) * 4 + c) * 4);
     if (MASK) {
       const int k = key0 + 16 * b + 2 * c;
       if (k >= len) w &= 0xffffff00u;
@@ -272,9 +275,9 @@ __device__ __forceinline__ void step(Acc<D, NT>& acc, uint32_t blk, uint32_t sq,
       // bytes of one channel's codes of two tokens: even channels, odd channels
       const uint32_t m = 0x0f0f0f0fu;
       uint32_t e0[4], o0[4], e1[4], o1[4];
-      codes_to_half2((v0[j] & m) | ((v0[W2 + j] & m) << 4), e0);
+      codes_to_half2((v0[j] & m) | ((v0[W2 + j] << 4) & ~m), e0);
       codes_to_half2(((v0[j] >> 4) & m) | (v0[W2 + j] & ~m), o0);
-      codes_to_half2((v1[j] & m) | ((v1[W2 + j] & m) << 4), e1);
+      codes_to_half2((v1[j] & m) | ((v1[W2 + j] << 4) & ~m), e1);
       codes_to_half2(((v1[j] >> 4) & m) | (v1[W2 + j] & ~m), o1);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -287,31 +290,145 @@ __device__ __forceinline__ void step(Acc<D, NT>& acc, uint32_t blk, uint32_t sq,
   }
 }
 
-__device__ __forceinline__ long long range_start(long long total, int blocks, int c) { return total * c / blocks; }
-// The block whose range holds `at`: the largest c with total * c / blocks <= at.
-__device__ __forceinline__ int range_owner(long long at, long long total, int blocks) {
-  return static_cast<int>(((at + 1) * blocks - 1) / total);
-}
+// The line of `total` steps in `blocks` runs: run c starts at total * c / blocks,
+// so that equal units which the blocks divide evenly are cut where they end.
+struct Split {
+  int total, blocks, per, more;
+  __device__ __forceinline__ Split(int total_, int blocks_)
+      : total(total_), blocks(blocks_), per(total_ / blocks_), more(total_ - per * blocks_) {}
+  __device__ __forceinline__ int start(int c) const { return c * per + c * more / blocks; }
+  // the run that holds step `at`
+  __device__ __forceinline__ int owner(int at) const {
+    int c = min(blocks - 1, static_cast<int>(static_cast<float>(at) * blocks / total));  // off by one or two
+    while (c > 0 && start(c) > at) --c;
+    while (c + 1 < blocks && start(c + 1) <= at) ++c;
+    return c;
+  }
+};
 
 template <bool BF16>
 __device__ __forceinline__ void store4(uint16_t* dst, float4 x) {
   *reinterpret_cast<uint2*>(dst) = make_uint2(float2_to_pair<BF16>(x.x, x.y), float2_to_pair<BF16>(x.z, x.w));
 }
 
+// Joins the pieces of a unit: the second slot of the block that starts it and
+// the first slots of those after it. Whole block; `red` is free shared memory.
 template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) cache4_few_kernel(const FewParams p) {
+__device__ __forceinline__ void join(const FewParams& p, float* red, int first_block, int pieces, int first, int row0,
+                                     int nrows, int head, float vf) {
+  constexpr int ROWS = 8 * NT, V = D / 32;  // V channels of a lane
+  constexpr int WARPS = Few<D, NT>::WARPS;
+  const AttnParams& a = p.a;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  // a warp per row and turn; where warps would be left over, several share a row's pieces
+  int parts = 1;
+  while (parts * 2 * nrows <= WARPS) parts *= 2;
+  const int part = warp % parts;
+  auto slot_row = [&](int k, int row) -> long long {
+    return (k == 0 ? first_block * 2ll + 1 : (static_cast<long long>(first_block) + k) * 2) * ROWS + row;
+  };
+  for (int row = warp / parts; row < (parts > 1 ? WARPS / parts : nrows); row += WARPS / parts) {
+    const bool there = row < nrows;
+    float m = -INFINITY, l = 0.f, x[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = 0.f;
+    // the pieces of this warp, 32 at a time and eight at once: lane i has the
+    // (m, l) of the i-th, which is loaded together with the first eight's sums
+    for (int k0 = part; there && k0 < pieces; k0 += 32 * parts) {
+      const int here = min(32, (pieces - k0 + parts - 1) / parts);
+      float2 u = make_float2(-INFINITY, 0.f);
+      if (lane < here) u = __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot_row(k0 + lane * parts, row) * 2));
+      float w = 0.f;
+      for (int i0 = 0; i0 < here; i0 += 8) {
+        float y[8][V];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float* src = p.part_o + slot_row(k0 + min(i0 + i, here - 1) * parts, row) * D + lane * V;
+          if (V == 4)
+            *reinterpret_cast<float4*>(y[i]) = __ldcg(reinterpret_cast<const float4*>(src));
+          else
+            *reinterpret_cast<float2*>(y[i]) = __ldcg(reinterpret_cast<const float2*>(src));
+        }
+        if (i0 == 0) {
+          float mx = u.x;
+#pragma unroll
+          for (int d = 16; d > 0; d /= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          if (mx > m) {
+            const float alpha = fa::ex2_approx(m - mx);
+            l *= alpha;
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] *= alpha;
+            m = mx;
+          }
+          w = u.x == -INFINITY ? 0.f : fa::ex2_approx(u.x - m);
+          l += u.y * w;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float f = __shfl_sync(0xffffffffu, w, i0 + i);
+          if (i0 + i < here) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] += y[i][e] * f;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
+    if (parts > 1) {  // one turn, all warps
+#pragma unroll
+      for (int e = 0; e < V; ++e) red[warp * (D + 2) + lane * V + e] = x[e];
+      if (lane == 0) {
+        red[warp * (D + 2) + D] = m;
+        red[warp * (D + 2) + D + 1] = l;
+      }
+      __syncthreads();
+      if (part == 0) {
+        float all = m;
+        for (int k = 1; k < parts; ++k) all = fmaxf(all, red[(warp + k) * (D + 2) + D]);
+        const float f0 = m == -INFINITY ? 0.f : fa::ex2_approx(m - all);
+        l *= f0;
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] *= f0;
+        m = all;
+        for (int k = 1; k < parts; ++k) {
+          const float* from = red + (warp + k) * (D + 2);
+          const float f = from[D] == -INFINITY ? 0.f : fa::ex2_approx(from[D] - all);
+          l += from[D + 1] * f;
+#pragma unroll
+          for (int e = 0; e < V; ++e) x[e] += from[lane * V + e] * f;
+        }
+      }
+    }
+    if (there && part == 0) {
+      const float inv = m == -INFINITY ? 0.f : vf / l;
+      const int t = (row0 + row) / a.group, g = (row0 + row) % a.group;
+      uint16_t* dst = a.o + (first + t) * a.o_stride_t + (static_cast<long long>(head) * a.group + g) * a.o_stride_h +
+                      lane * V;
+#pragma unroll
+      for (int e = 0; e < V; e += 2)
+        *reinterpret_cast<uint32_t*>(dst + e) = float2_to_pair<BF16>(x[e] * inv, x[e + 1] * inv);
+    }
+  }
+}
+
+template <int D, int NT, bool BF16>
+__global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache4_few_kernel(const FewParams p) {
   using C = Few<D, NT>;
   using L = Layout<D>;
+  constexpr int WARPS = C::WARPS, THREADS = C::THREADS;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ long long chunk_before[MAX_CHUNKS + 1];
-  __shared__ long long warp_part[WARPS];
-  __shared__ long long found_base;
-  __shared__ int found_r;
+  __shared__ int chunk_before[C::MAX_CHUNKS];
+  __shared__ int weight_part[WARPS], unit_part[WARPS], weight_high[WARPS];
+  __shared__ Share found;
+  __shared__ int found_base, found_r;
+  __shared__ bool joins;
   const AttnParams& a = p.a;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int n = lane >> 2, c = lane & 3;
   const uint32_t s0 = fa::smem_u32(smem);
   const uint32_t ring = s0 + warp * C::RING;
+  const uint8_t* ring_at = smem + warp * C::RING;
   float2* ml = reinterpret_cast<float2*>(smem + C::ML_OFF);
   float* rowf = reinterpret_cast<float*>(smem + C::ROWF_OFF);
   fa::griddep_wait();
@@ -319,69 +436,98 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) cache4_few_kernel(co
 
   // ---- this block's part [pos, end) of the line of steps
   const int chunks = (a.requests + THREADS - 1) / THREADS;
-  long long total = 0;
+  long long total64 = 0;
+  int units = 0;
+  Share mine{};
   for (int k = 0; k < chunks; ++k) {
     const int r = k * THREADS + threadIdx.x;
-    long long w = r < a.requests ? share_of<C::ROWS>(p, r).weight : 0;
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) w += __shfl_xor_sync(0xffffffffu, w, d);
-    if (lane == 0) warp_part[warp] = w;
+    mine = Share{};
+    if (r < a.requests) mine = share_of<C::ROWS>(p, r);
+    // a request's weight fits 31 bits (the host sees to it), their sum may not,
+    // if query_start decreases somewhere: it is added up in two halves
+    const unsigned weight = static_cast<unsigned>(mine.units) * mine.steps;
+    const unsigned low = __reduce_add_sync(0xffffffffu, weight & 0xffffu);
+    const unsigned high = __reduce_add_sync(0xffffffffu, weight >> 16);
+    const unsigned u = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(mine.units));
+    if (lane == 0) {
+      weight_part[warp] = low;
+      weight_high[warp] = high;
+      unit_part[warp] = u;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) chunk_before[k] = total;
+    if (threadIdx.x == 0) chunk_before[k] = static_cast<int>(total64);
 #pragma unroll
-    for (int i = 0; i < WARPS; ++i) total += warp_part[i];
+    for (int i = 0; i < WARPS; ++i) {
+      total64 += (static_cast<long long>(weight_high[i]) << 16) + weight_part[i];
+      units += unit_part[i];
+    }
     __syncthreads();
   }
-  const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + MIN_STEPS - 1) / MIN_STEPS));
-  JoinRecord rec{};
-  long long pos = 0, end = 0;
+  if (total64 > INT_MAX) total64 = 0;
+  const int total = static_cast<int>(total64);
+  // as many blocks as there are, or as many for each unit as its steps are
+  // worth: equal units are then cut into equal pieces, or not at all
+  int blocks = gridDim.x;
+  if (total < blocks * C::MIN_STEPS) blocks = total ? min(blocks, units * max(1, total / units / C::MIN_STEPS)) : 0;
+  const Split split(total, max(blocks, 1));
+  int pos = 0, end = 0;
   if (static_cast<int>(blockIdx.x) < blocks) {
-    pos = range_start(total, blocks, blockIdx.x);
-    end = range_start(total, blocks, blockIdx.x + 1);
+    pos = split.start(blockIdx.x);
+    end = split.start(blockIdx.x + 1);
   }
-  int r = 0;
-  long long base = 0;
+  int r = 0, base = 0;
+  Share sh{};
   if (pos < end) {
     int k = 0;
     while (k + 1 < chunks && chunk_before[k + 1] <= pos) ++k;
-    const int rr = k * THREADS + threadIdx.x;
-    const long long w = rr < a.requests ? share_of<C::ROWS>(p, rr).weight : 0;
-    long long inc = w;
+    r = k * THREADS + threadIdx.x;
+    if (chunks > 1) mine = r < a.requests ? share_of<C::ROWS>(p, r) : Share{};
+    const int w = mine.units * mine.steps;
+    int inc = w;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
-      const long long y = __shfl_up_sync(0xffffffffu, inc, d);
+      const int y = __shfl_up_sync(0xffffffffu, inc, d);
       if (lane >= d) inc += y;
     }
-    if (lane == 31) warp_part[warp] = inc;
+    if (lane == 31) unit_part[warp] = inc;
     __syncthreads();
-    long long before = chunk_before[k] + inc - w;
-    for (int i = 0; i < warp; ++i) before += warp_part[i];
-    if (before <= pos && pos < before + w) {
+    int before = chunk_before[k] + inc - w;
+    for (int i = 0; i < warp; ++i) before += unit_part[i];
+    if (before <= pos && pos - before < w) {
+      found = mine;
       found_base = before;
-      found_r = rr;
+      found_r = r;
     }
     __syncthreads();
-    r = found_r;
+    sh = found;
     base = found_base;
+    r = found_r;
   }
 
   while (pos < end) {
-    const Share sh = share_of<C::ROWS>(p, r);
-    if (pos >= base + sh.weight) {  // the next request (the line ends with the last one's units)
-      base += sh.weight;
+    if (pos - base >= sh.units * sh.steps) {  // the next request (the line ends with the last one's units)
+      base += sh.units * sh.steps;
       ++r;
+      sh = share_of<C::ROWS>(p, r);
       continue;
     }
-    const Rows rows = rows_of(a, r);
-    const int len = length_of(a, r);
-    const long long unit = (pos - base) / sh.steps;
-    const int off = static_cast<int>((pos - base) % sh.steps);
-    const int stop = static_cast<int>(min(static_cast<long long>(sh.steps), off + (end - pos)));
-    const int head = static_cast<int>(unit % a.kv_heads);
-    const int row0 = static_cast<int>(unit / a.kv_heads) * C::ROWS;
-    const int nrows = min(C::ROWS, rows.n * a.group - row0);
+    const int unit = (pos - base) / sh.steps;
+    const int off = pos - base - unit * sh.steps;
+    const int stop = min(sh.steps, off + end - pos);
+    const int head = unit % a.kv_heads;
+    const int row0 = unit / a.kv_heads * C::ROWS;
+    const int nrows = min(C::ROWS, sh.rows - row0);
+    const int len = sh.len, tokens = sh.rows / a.group;
     const int k_begin = max(off, 1) - 1, k_end = stop - 1;  // steps that hold keys
     const int* table = a.tables + static_cast<long long>(r) * a.width;
+    const bool starts = off == 0, ends = stop == sh.steps;
+    const int first_block = starts ? static_cast<int>(blockIdx.x) : split.owner(pos - off);
+    const float kf = a.scale_log2 * (a.k_scale ? a.k_scale[head] : 1.f);
+    const float vf = a.v_scale ? a.v_scale[head] : 1.f;
+    unsigned long long* count = p.done + first_block;
+    // the unit's count is looked at here, and set up long before it is needed
+    unsigned long long count_was = p.epoch << 16;
+    if (!(starts && ends) && threadIdx.x == 0) count_was = *reinterpret_cast<volatile unsigned long long*>(count);
 
     // ---- copies of this warp's first steps
     int page_ids = 0, ids_at = -32;  // page of step k_begin + warp + WARPS * (ids_at + lane)
@@ -425,7 +571,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) cache4_few_kernel(co
         uint4 x = make_uint4(0, 0, 0, 0);
         if (row < nrows) {
           const int t = (row0 + row) / a.group, g = (row0 + row) % a.group;
-          x = *reinterpret_cast<const uint4*>(a.q + (rows.first + t) * a.q_stride_t +
+          x = *reinterpret_cast<const uint4*>(a.q + (sh.first + t) * a.q_stride_t +
                                               (static_cast<long long>(head) * a.group + g) * a.q_stride_h + ch * 8);
         }
         float f = 1.f;
@@ -460,12 +606,12 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) cache4_few_kernel(co
         *reinterpret_cast<uint4*>(smem + C::Q_OFF + (((row / 8) * (D / 32) + ch % (D / 32)) * 32 + lane_to) * 16) = x;
       }
     }
+    if ((count_was >> 16) != p.epoch) atomicCAS(count, count_was, p.epoch << 16);
     __syncthreads();
 
     Acc<D, NT> acc;
     float factor[NT][2];
     int limit[NT][2];
-    const float kf = a.scale_log2 * (a.k_scale ? a.k_scale[head] : 1.f);
     int least = INT_MAX;  // first token that some row of the unit does not see
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -473,11 +619,11 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) cache4_few_kernel(co
       for (int i = 0; i < 2; ++i) {
         const int row = nt * 8 + 2 * c + i;
         factor[nt][i] = kf * rowf[row];
-        limit[nt][i] = a.causal && row < nrows ? len - rows.n + 1 + (row0 + row) / a.group : len;
+        limit[nt][i] = a.causal && row < nrows ? len - tokens + 1 + (row0 + row) / a.group : len;
         acc.m[nt][i] = -INFINITY;
         acc.l[nt][i] = 0.f;
       }
-    least = a.causal ? min(len, len - rows.n + 1 + row0 / a.group) : len;
+    least = a.causal ? min(len, len - tokens + 1 + row0 / a.group) : len;
 #pragma unroll
     for (int t = 0; t < D / 16; ++t)
 #pragma unroll
@@ -494,9 +640,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) cache4_few_kernel(co
       if ((good >> stage) & 1u) {
         const int key0 = (k_begin + warp + WARPS * i) * STEP;
         if (key0 + STEP > least)
-          step<D, NT, true>(acc, ring + stage * C::STEP_BYTES, s0 + C::Q_OFF, lane, factor, key0, len, limit);
+          step<D, NT, true>(acc, ring_at + stage * C::STEP_BYTES, smem + C::Q_OFF, lane, factor, key0, len, limit);
         else
-          step<D, NT, false>(acc, ring + stage * C::STEP_BYTES, s0 + C::Q_OFF, lane, factor, key0, len, limit);
+          step<D, NT, false>(acc, ring_at + stage * C::STEP_BYTES, smem + C::Q_OFF, lane, factor, key0, len, limit);
       }
       __syncwarp();  // the stage is free for the next copy
     }
@@ -533,9 +679,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) cache4_few_kernel(co
               make_float2(acc.o[t][nt][i] * f, acc.o[t][nt][2 + i] * f);
       }
     __syncthreads();
-    const bool starts = off == 0, ends = stop == sh.steps;
     const long long slot = static_cast<long long>(blockIdx.x) * 2 + (starts ? 1 : 0);
-    const float vf = a.v_scale ? a.v_scale[head] : 1.f;
     for (int at = threadIdx.x; at < nrows * (D / 4); at += THREADS) {
       const int row = at / (D / 4), d = at % (D / 4) * 4;
       float m = -INFINITY, l = 0.f;
@@ -555,7 +699,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) cache4_few_kernel(co
       if (starts && ends) {
         const float inv = m == -INFINITY ? 0.f : vf / l;
         const int t = (row0 + row) / a.group, g = (row0 + row) % a.group;
-        store4<BF16>(a.o + (rows.first + t) * a.o_stride_t +
+        store4<BF16>(a.o + (sh.first + t) * a.o_stride_t +
                          (static_cast<long long>(head) * a.group + g) * a.o_stride_h + d,
                      make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
       } else {
@@ -563,98 +707,36 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3) cache4_few_kernel(co
         if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * C::ROWS + row) * 2) = make_float2(m, l);
       }
     }
-    if (starts && !ends) {
-      const int last = range_owner(pos - off + sh.steps - 1, total, blocks);
-      rec = {last - static_cast<int>(blockIdx.x) + 1, rows.first, row0, nrows, head, {0, 0, 0}};
+    if (!(starts && ends)) {
+      // The block that finishes the unit's last piece joins them, in their
+      // order whoever it is. The barrier orders the block's stores before
+      // thread 0's fence, and that before its count.
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const int pieces = split.owner(pos - off + sh.steps - 1) - first_block + 1;
+        __threadfence();
+        const int before = static_cast<int>(atomicAdd(count, 1ull) & 0xffffull);
+        joins = before + 1 == pieces;
+        if (joins) {
+          __threadfence();
+          atomicExch(count, p.epoch << 16);
+        }
+      }
+      __syncthreads();
+      if (joins)
+        join<D, NT, BF16>(p, reinterpret_cast<float*>(smem), first_block,
+                          split.owner(pos - off + sh.steps - 1) - first_block + 1, sh.first, row0, nrows, head, vf);
     }
     pos += stop - off;
     __syncthreads();  // the merge buffers, Q and row factors are free
   }
-  if (threadIdx.x == 0) p.record[blockIdx.x] = rec;
-}
-
-// Joins the pieces of the unit that block blockIdx.x started and did not end:
-// its own second slot and the first slots of the blocks after it, in that
-// order. Also zeroes the rows behind the last request, when asked to.
-template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(256) cache4_join_kernel(const FewParams p) {
-  constexpr int ROWS = 8 * NT;
-  constexpr int V = D / 32;  // channels of a lane
-  __shared__ float red[8][D + 2];
-  const AttnParams& a = p.a;
-  fa::griddep_wait();
-  if (threadIdx.x == 0) fa::griddep_launch_dependents();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (a.zero_rest) {
     const int from = min(max(a.query_start[a.requests], 0), a.tokens);
     const long long per = static_cast<long long>(a.kv_heads) * a.group * (D / 4);
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < (a.tokens - from) * per; i += gridDim.x * 256ll) {
+    for (long long i = static_cast<long long>(blockIdx.x) * THREADS + threadIdx.x; i < (a.tokens - from) * per;
+         i += static_cast<long long>(gridDim.x) * THREADS) {
       const long long t = from + i / per, h = i % per / (D / 4);
       store4<BF16>(a.o + t * a.o_stride_t + h * a.o_stride_h + i % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-    }
-  }
-  const JoinRecord rec = p.record[blockIdx.x];
-  if (rec.pieces == 0) return;
-  // 8 warps: `parts` of them share a row's pieces
-  const int parts = rec.rows <= 1 ? 8 : rec.rows <= 2 ? 4 : rec.rows <= 4 ? 2 : 1;
-  const int part = warp % parts;
-  const float vf = a.v_scale ? a.v_scale[rec.head] : 1.f;
-  for (int row = warp / parts; row < (rec.rows + 8 / parts - 1) / (8 / parts) * (8 / parts); row += 8 / parts) {
-    const bool there = row < rec.rows;
-    auto slot_row = [&](int k) -> long long {
-      const long long slot = k == 0 ? blockIdx.x * 2ll + 1 : (static_cast<long long>(blockIdx.x) + k) * 2;
-      return slot * ROWS + row;
-    };
-    float m = -INFINITY, l = 0.f, x[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) x[e] = 0.f;
-    if (there) {
-      for (int k = lane; k < rec.pieces; k += 32) m = fmaxf(m, p.part_ml[slot_row(k) * 2]);
-#pragma unroll
-      for (int d = 16; d > 0; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-      if (m > -INFINITY) {
-#pragma unroll 4
-        for (int k = part; k < rec.pieces; k += parts) {
-          const long long at = slot_row(k);
-          const float2 u = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-          const float f = u.x == -INFINITY ? 0.f : fa::ex2_approx(u.x - m);
-          l += u.y * f;
-          if (V == 4) {
-            const float4 y = *reinterpret_cast<const float4*>(p.part_o + at * D + lane * V);
-            x[0] += y.x * f;
-            x[1] += y.y * f;
-            x[V - 2] += y.z * f;
-            x[V - 1] += y.w * f;
-          } else {
-            const float2 y = *reinterpret_cast<const float2*>(p.part_o + at * D + lane * V);
-            x[0] += y.x * f;
-            x[1] += y.y * f;
-          }
-        }
-      }
-    }
-    if (parts > 1) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) red[warp][lane * V + e] = x[e];
-      if (lane == 0) red[warp][D] = l;
-      __syncthreads();
-      if (part == 0) {
-        for (int k = 1; k < parts; ++k) {
-#pragma unroll
-          for (int e = 0; e < V; ++e) x[e] += red[warp + k][lane * V + e];
-          l += red[warp + k][D];
-        }
-      }
-      __syncthreads();
-    }
-    if (there && part == 0) {
-      const float inv = m == -INFINITY ? 0.f : vf / l;
-      const int t = (rec.row0 + row) / a.group, g = (rec.row0 + row) % a.group;
-      uint16_t* dst = a.o + (rec.first + t) * a.o_stride_t +
-                      (static_cast<long long>(rec.head) * a.group + g) * a.o_stride_h + lane * V;
-#pragma unroll
-      for (int e = 0; e < V; e += 2)
-        *reinterpret_cast<uint32_t*>(dst + e) = float2_to_pair<BF16>(x[e] * inv, x[e + 1] * inv);
     }
   }
 }
@@ -662,7 +744,7 @@ __global__ void __launch_bounds__(256) cache4_join_kernel(const FewParams p) {
 // -------------------------------------------------------------------- host
 static bool args_ok(const gfx906_b200_cache4_attn_args& g) {
   return g.dtype >= 0 && g.dtype <= 1 && g.tokens >= 0 && g.heads > 0 && g.kv_heads > 0 && g.heads % g.kv_heads == 0 &&
-         g.pages >= 0 && g.requests >= 0 && g.requests <= MAX_CHUNKS * THREADS && g.width >= 0 &&
+         g.pages >= 0 && g.requests >= 0 && g.requests <= MAX_REQUESTS && g.width >= 0 &&
          g.width <= INT_MAX / PAGE && g.max_tokens >= 0 && isfinite(g.scale) &&
          static_cast<long long>(g.tokens) * (g.heads / g.kv_heads) <= INT_MAX;
 }
@@ -670,18 +752,26 @@ static bool args_ok(const gfx906_b200_cache4_attn_args& g) {
 struct Plan {
   int nt;      // row tiles of 8 NT rows
   int blocks;
-  size_t ml_off, rec_off, many_off, bytes;
+  size_t ml_off, done_off, many_off, bytes;
+  bool fits;
   ManyPlan many;  // max_blocks 0: no request has that many rows
 };
 static Plan plan_of(const gfx906_b200_cache4_attn_args& g, int sms) {
   Plan pl{};
   const long long rows = static_cast<long long>(g.max_tokens) * (g.heads / g.kv_heads);
   pl.nt = rows <= 8 ? 1 : 2;
-  pl.blocks = sms * (pl.nt == 1 ? 4 : 3);
+  pl.blocks = sms * (pl.nt == 1 ? Few<128, 1>::PER_SM : Few<128, 2>::PER_SM);
+  // the line of steps is counted in 31 bits
+  const long long tiles = rows > FEW_ROWS ? static_cast<long long>(g.requests) * (FEW_ROWS / (8 * pl.nt))
+                                          : static_cast<long long>(g.tokens) * (g.heads / g.kv_heads) / (8 * pl.nt) + g.requests;
+  pl.fits = tiles * g.kv_heads <= INT_MAX / (2ll * g.width + 2);
+  // no more blocks than the tables can hold steps for
+  const long long most = pl.fits ? tiles * g.kv_heads * max(1ll, (2ll * g.width + 1) / Few<128, 1>::MIN_STEPS) : 1;
+  pl.blocks = static_cast<int>(min(static_cast<long long>(pl.blocks), max(1ll, most)));
   const size_t slots = static_cast<size_t>(pl.blocks) * 2 * 8 * pl.nt;
   pl.ml_off = slots * g.D * sizeof(float);
-  pl.rec_off = pl.ml_off + slots * 2 * sizeof(float);
-  pl.many_off = (pl.rec_off + pl.blocks * sizeof(JoinRecord) + 255) & ~static_cast<size_t>(255);
+  pl.done_off = pl.ml_off + slots * 2 * sizeof(float);
+  pl.many_off = (pl.done_off + pl.blocks * sizeof(unsigned long long) + 255) & ~static_cast<size_t>(255);
   if (rows > FEW_ROWS) pl.many = many_plan(g.tokens, g.requests, g.heads / g.kv_heads, g.kv_heads, g.D, sms);
   pl.bytes = pl.many_off + ((pl.many.bytes + 255) & ~static_cast<size_t>(255));
   return pl;
@@ -689,12 +779,9 @@ static Plan plan_of(const gfx906_b200_cache4_attn_args& g, int sms) {
 
 template <int D, int NT, bool BF16>
 static int launch_few(const FewParams& p, int blocks, cudaStream_t stream) {
-  const cudaError_t e = cudaFuncSetAttribute(cache4_few_kernel<D, NT, BF16>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, Few<D, NT>::SMEM);
-  if (e != cudaSuccess) return GFX906_B200_ECUDA;
-  const int rc = launch(cache4_few_kernel<D, NT, BF16>, dim3(blocks), dim3(THREADS), Few<D, NT>::SMEM, stream, p);
-  if (rc != GFX906_B200_OK) return rc;
-  return launch(cache4_join_kernel<D, NT, BF16>, dim3(blocks), dim3(256), 0, stream, p);
+  static SmemAttribute smem;
+  if (!smem.set(cache4_few_kernel<D, NT, BF16>, Few<D, NT>::SMEM)) return GFX906_B200_ECUDA;
+  return launch(cache4_few_kernel<D, NT, BF16>, dim3(blocks), dim3(Few<D, NT>::THREADS), Few<D, NT>::SMEM, stream, p);
 }
 template <int D, int NT>
 static int launch_few_t(const FewParams& p, int dtype, int blocks, cudaStream_t stream) {
@@ -715,7 +802,7 @@ static int attn(const gfx906_b200_cache4_attn_args& g, void* ws, size_t ws_bytes
   const int rc = gfx906_b200_internal_device(&sms);
   if (rc != GFX906_B200_OK) return rc;
   const Plan pl = plan_of(g, sms);
-  if (!ws || ws_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(ws) & 255u)) return GFX906_B200_EINVAL;
+  if (!pl.fits || (static_cast<long long>(g.max_tokens) * (g.heads / g.kv_heads) > FEW_ROWS && !pl.many.max_blocks) || !ws || ws_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(ws) & 255u)) return GFX906_B200_EINVAL;
   FewParams p{};
   p.a = {static_cast<const uint16_t*>(g.q), static_cast<uint16_t*>(g.o), static_cast<const uint8_t*>(g.cache), g.tables,
          g.lengths, g.query_start, g.k_scale, g.v_scale, g.q_stride_t, g.q_stride_h, g.o_stride_t, g.o_stride_h,
@@ -737,7 +824,8 @@ static int attn(const gfx906_b200_cache4_attn_args& g, void* ws, size_t ws_bytes
   }
   p.part_o = reinterpret_cast<float*>(base);
   p.part_ml = reinterpret_cast<float*>(base + pl.ml_off);
-  p.record = reinterpret_cast<JoinRecord*>(base + pl.rec_off);
+  p.done = reinterpret_cast<unsigned long long*>(base + pl.done_off);
+  p.epoch = gfx906_b200_internal_next_epoch() & 0xffffffffffffull;
   if (g.D == 128)
     return pl.nt == 1 ? launch_few_t<128, 1>(p, g.dtype, pl.blocks, stream)
                       : launch_few_t<128, 2>(p, g.dtype, pl.blocks, stream);

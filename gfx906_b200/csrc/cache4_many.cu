@@ -44,6 +44,7 @@ constexpr uint32_t M_REGS_SOFTMAX = 192;
 constexpr uint32_t M_REGS_CONVERT = 96;
 constexpr uint32_t M_REGS_ISSUE = 32;
 constexpr float M_RESCALE = 8.0f;    // log2 units, see the dense kernels
+constexpr float M_LARGE = 67108864.f;  // 2^26: half a 32-bit step is 2 log2 units
 
 __device__ unsigned int g_cache4_status = 0;  // 1: a wait ran out
 
@@ -492,7 +493,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
         holes |= static_cast<unsigned>(__ldg(table + i)) >= static_cast<unsigned>(a.pages);
       holes = __any_sync(0xffffffffu, holes);
       float m = -INFINITY, l = 0.f;
-      bool ok = true;
+      bool ok = true, large = false;
       for (int j = t0; j < t1; ++j) {
         const uint32_t parity = (j - t0) & 1;
         if (!wait(C::B_S + ti, parity)) { ok = false; break; }
@@ -521,15 +522,27 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
           f = ex2_approx(m - m_new);
           m = m_new;
         }
-        rescale_rows<D>(tO, j > t0 && __any_sync(0xffffffffu, need), f);
-        l *= f;
-        const float neg_m = m == -INFINITY ? 0.f : -m;
+        if (__any_sync(0xffffffffu, need)) {
+          rescale_rows<D>(tO, j > t0, f);
+          l *= f;
+          large = __any_sync(0xffffffffu, fabsf(m) > M_LARGE && m > -INFINITY);
+        }
+        float neg_m = m == -INFINITY ? 0.f : -m, mul = sl2;
+        if (large) {
+          // Scores so large that m is a rounded product: round each score as m
+          // was, or the largest would lie half a step of m above or below it.
+#pragma unroll
+          for (int c = 0; c < BN; ++c)
+            s[c] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(s[c]), sl2), neg_m));
+          mul = 1.f;
+          neg_m = 0.f;
+        }
         const uint32_t half_bar = bars + 8 * (C::B_P_HALF + ti);
         float sum0, sum1;
         if (full)
-          row_exp_store<false>(s, sl2, neg_m, hi, tS, sum0, sum1, half_bar, [] {}, [] {});
+          row_exp_store<false>(s, mul, neg_m, hi, tS, sum0, sum1, half_bar, [] {}, [] {});
         else
-          row_exp_store<true>(s, sl2, neg_m, hi, tS, sum0, sum1, half_bar, [] {}, [] {}, lo);
+          row_exp_store<true>(s, mul, neg_m, hi, tS, sum0, sum1, half_bar, [] {}, [] {}, lo);
         l += sum0 + sum1;
         tmem_wait_st();
         tc_fence_before();
@@ -673,9 +686,8 @@ ManyPlan many_plan(int tokens, int requests, int group, int kv_heads, int D, int
 
 template <int D, bool BF16>
 static int launch_many_t(const ManyParams& p, cudaStream_t stream) {
-  const cudaError_t e = cudaFuncSetAttribute(cache4_many_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             Many<D>::SMEM);
-  if (e != cudaSuccess) return GFX906_B200_ECUDA;
+  static SmemAttribute smem;
+  if (!smem.set(cache4_many_kernel<D, BF16>, Many<D>::SMEM)) return GFX906_B200_ECUDA;
   const int units = p.max_blocks * p.a.kv_heads;
   const int rc = launch(cache4_many_kernel<D, BF16>, dim3(units * p.pieces), dim3(M_THREADS), Many<D>::SMEM, stream, p);
   if (rc != GFX906_B200_OK || p.pieces == 1) return rc;

@@ -322,16 +322,12 @@ __global__ void __launch_bounds__(256) cache4_read_kernel(const ReadParams p) {
 }
 
 // -------------------------------------------------------------------- host
-static int plan_smem_attribute() {
-  const cudaError_t e = cudaFuncSetAttribute(cache4_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             PLAN_MAX_REQUESTS * 5 * static_cast<int>(sizeof(int)));
-  return e == cudaSuccess ? GFX906_B200_OK : GFX906_B200_ECUDA;
-}
-
 static int plan(const PlanParams& p, cudaStream_t stream) {
-  int sms = 0, rc = gfx906_b200_internal_device(&sms);
-  if (rc == GFX906_B200_OK) rc = plan_smem_attribute();
+  int sms = 0;
+  const int rc = gfx906_b200_internal_device(&sms);
   if (rc != GFX906_B200_OK) return rc;
+  static SmemAttribute smem;
+  if (!smem.set(cache4_plan_kernel, PLAN_MAX_REQUESTS * 5 * static_cast<int>(sizeof(int)))) return GFX906_B200_ECUDA;
   // a block for every 1024 tokens or 32 requests
   const int blocks = min(sms, 1 + max(p.tokens / 1024, p.requests / 32));
   return launch(cache4_plan_kernel, dim3(blocks), dim3(PLAN_THREADS), static_cast<size_t>(p.requests) * 5 * sizeof(int),

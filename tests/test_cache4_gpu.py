@@ -334,6 +334,20 @@ def test_attention_many_tokens_bad_pages_nan_queries_and_strides():
     p.check(out, causal=False, rows=[0, 7, 8, 127, 128, 139, 199])
 
 
+def test_attention_many_tokens_enormous_scores():
+    """bf16 rows of any size: beyond 32 bits of score the largest one takes all."""
+    p = Problem([130], [300], 1, 1, 128, torch.bfloat16)
+    p.q[::2] *= 2.0 ** 60
+    p.q[1] *= 2.0 ** -100
+    out = p.run(causal=False)
+    k, v = p.k[0][:, 0].double(), p.v[0][:, 0].double()
+    for i in range(0, 130, 2):
+        best = (k @ p.q[i, 0].double()).argmax()
+        assert (out[i, 0].cpu().double() - v[best]).abs().max() <= 2.0 ** -8 * v[best].abs().max(), i
+    p.q[::2] = 0
+    p.check(p.run(causal=False), causal=False, rows=[0, 1, 2, 3, 129])
+
+
 def test_attention_many_tokens_growing_scores():
     """Scores that grow along the keys move every row's maximum again and again."""
     p = Problem([130], [700], 1, 1, 64, torch.float16)
