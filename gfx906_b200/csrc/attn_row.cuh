@@ -61,11 +61,13 @@ __device__ __forceinline__ float row_extreme(const uint32_t* s, int nvalid, bool
 // fp32 row sum in two partial sums. EMU_PAIRS of every 4 column pairs use the
 // FMA-pipe polynomial, the rest MUFU. MASK zeroes columns outside [lo,
 // nvalid) (last key tile).
+// TWO_STEPS rounds the product before neg_m is added, as a maximum that was
+// computed by itself was rounded.
 // When half_bar is non-zero, the first half of P (keys 0..63) is published on
 // it as soon as it is stored (after before_half() has run), so the tensor core
 // can start on those keys while the second half is computed. before_store()
 // runs once, after the first half's exponentials and before any of P is stored.
-template <bool MASK, typename BeforeHalf, typename BeforeStore>
+template <bool MASK, bool TWO_STEPS = false, typename BeforeHalf, typename BeforeStore>
 __device__ __forceinline__ void row_exp_store(const uint32_t* s, float sl2, float neg_m, int nvalid,
                                               uint32_t tS, float& sum0, float& sum1, uint32_t half_bar,
                                               BeforeHalf&& before_half, BeforeStore&& before_store, int lo = 0) {
@@ -78,9 +80,13 @@ __device__ __forceinline__ void row_exp_store(const uint32_t* s, float sl2, floa
 #pragma unroll
     for (int c2 = 0; c2 < 32; ++c2) {
       const int c = h * 64 + 2 * c2;
-      const uint64_t X = f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sl2x2, negm2);
       float x0, x1, e0, e1;
-      f2_unpack(X, x0, x1);
+      if (TWO_STEPS) {
+        x0 = __fadd_rn(__fmul_rn(__uint_as_float(s[c]), sl2), neg_m);
+        x1 = __fadd_rn(__fmul_rn(__uint_as_float(s[c + 1]), sl2), neg_m);
+      } else {
+        f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sl2x2, negm2), x0, x1);
+      }
       if ((c2 & 3) < EMU_PAIRS) {
         exp2_poly3_x2(x0, x1, e0, e1);
       } else {

@@ -3,6 +3,8 @@
 // the current stream of their device, and failures raise RuntimeError.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <optional>
@@ -62,6 +64,36 @@ Tensor with_rows(const Tensor& t) {
   return rows_ok(c) ? c : c.clone();  // a contiguous view may start off 16 bytes
 }
 
+// These calls are as short as their launches, so results are allocated without
+// the dispatcher, and several of one type at once.
+Tensor new_tensor(c10::IntArrayRef sizes, c10::ScalarType type, const Tensor& on) {
+  return at::detail::empty_cuda(sizes, type, on.device(), std::nullopt);
+}
+// A contiguous tensor in `all`, from element `at` on.
+Tensor part_of(const Tensor& all, int64_t at, c10::IntArrayRef sizes) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(all.storage()), all.key_set(),
+                                                      all.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(at);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
+
+// Scratch memory of one call, from the caching allocator: calls on other streams
+// and other captured graphs never share it.
+class Workspace {
+ public:
+  Workspace(size_t bytes, cudaStream_t stream)
+      : p_(bytes ? c10::cuda::CUDACachingAllocator::raw_alloc_with_stream(bytes, stream) : nullptr) {}
+  ~Workspace() {
+    if (p_) c10::cuda::CUDACachingAllocator::raw_delete(p_);
+  }
+  Workspace(const Workspace&) = delete;
+  void* get() const { return p_; }
+
+ private:
+  void* p_;
+};
+
 void check_status(int rc) { TORCH_CHECK(rc == GFX906_B200_OK, "cache4: ", gfx906_b200_attn_error_string(rc)); }
 
 }  // namespace
@@ -81,16 +113,11 @@ PlanOut cache4_plan(Tensor tables, Tensor lengths, Tensor counts, Tensor free_pa
   TORCH_CHECK(W <= INT32_MAX / kPage && R * W <= INT32_MAX && free_pages.size(0) <= INT32_MAX, "cache4: sizes are too large");
   TORCH_CHECK(tokens >= 0 && tokens < INT32_MAX, "cache4: tokens must be a non-negative int32");
   const c10::cuda::CUDAGuard guard(tables.device());
-  // One allocation cut into the six results: a decoding step is bound by its launches.
-  const Tensor all = torch::empty({3 * R + 2 * tokens + 2}, tables.options());
+  const Tensor all = new_tensor({3 * R + 2 * tokens + 2}, torch::kInt32, tables);
   int64_t at = 0;
   auto cut = [&](int64_t n) {
-    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(all.storage()),
-                                                        all.key_set(), all.dtype());
-    t.unsafeGetTensorImpl()->set_storage_offset(at);
-    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
     at += n;
-    return t;
+    return part_of(all, at - n, {n});
   };
   Tensor query_start = cut(R + 1), lengths_out = cut(R), added = cut(R), slots = cut(tokens), positions = cut(tokens),
          free_out = cut(1);
@@ -129,9 +156,9 @@ std::tuple<Tensor, Tensor> cache4_read(Tensor cache, Tensor slots, std::optional
   const float* ks = check_scale(k_scale, cache, heads, "k_scale");
   const float* vs = check_scale(v_scale, cache, heads, "v_scale");
   const c10::cuda::CUDAGuard guard(cache.device());
-  const auto options =
-      cache.options().dtype(dtype == 0 ? torch::kHalf : dtype == 1 ? torch::kBFloat16 : torch::kFloat32);
-  Tensor k = torch::empty({slots.size(0), heads, D}, options), v = torch::empty_like(k);
+  const int64_t n = slots.size(0) * heads * D;
+  const Tensor all = new_tensor({2 * n}, dtype == 0 ? torch::kHalf : dtype == 1 ? torch::kBFloat16 : torch::kFloat32, cache);
+  Tensor k = part_of(all, 0, {slots.size(0), heads, D}), v = part_of(all, n, {slots.size(0), heads, D});
   check_status(gfx906_b200_cache4_read(cache.data_ptr(), pages, slots.data_ptr<int>(), ks, vs,
                                        static_cast<int>(slots.size(0)), heads, D, k.data_ptr(), v.data_ptr(),
                                        static_cast<int>(dtype), at::cuda::getCurrentCUDAStream()));
@@ -164,7 +191,7 @@ Tensor attn_cache4(Tensor q, Tensor cache, Tensor tables, Tensor lengths, Tensor
                 "cache4: out must be a tensor like q with rows that start on 16 bytes");
   const c10::cuda::CUDAGuard guard(cache.device());
   const Tensor qc = with_rows(q);
-  Tensor o = out.has_value() ? *out : torch::empty(q.sizes(), q.options());
+  Tensor o = out.has_value() ? *out : new_tensor(q.sizes(), q.scalar_type(), q);
   if (q.numel() == 0) return o;
   gfx906_b200_cache4_attn_args g{};
   g.q = qc.data_ptr();
@@ -191,11 +218,10 @@ Tensor attn_cache4(Tensor q, Tensor cache, Tensor tables, Tensor lengths, Tensor
   g.causal = causal ? 1 : 0;
   g.zero_rest = out.has_value() ? 0 : 1;
   g.scale = static_cast<float>(scale);
-  // A workspace of the call's own, from the caching allocator: calls on other
-  // streams and other captured graphs never share it.
+  const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const size_t bytes = gfx906_b200_cache4_attn_workspace_size(&g);
-  Tensor ws = torch::empty({static_cast<int64_t>(bytes)}, cache.options());
-  check_status(gfx906_b200_cache4_attn(&g, ws.data_ptr(), bytes, at::cuda::getCurrentCUDAStream()));
+  const Workspace ws(bytes, stream);
+  check_status(gfx906_b200_cache4_attn(&g, ws.get(), bytes, stream));
   return o;
 }
 

@@ -332,17 +332,17 @@ __device__ __forceinline__ void join(const FewParams& p, float* red, int first_b
     float m = -INFINITY, l = 0.f, x[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) x[e] = 0.f;
-    // the pieces of this warp, 32 at a time and eight at once: lane i has the
-    // (m, l) of the i-th, which is loaded together with the first eight's sums
+    // the pieces of this warp, 32 at a time and 16 at once: lane i has the
+    // (m, l) of the i-th, which is loaded together with the first 16 sums
     for (int k0 = part; there && k0 < pieces; k0 += 32 * parts) {
       const int here = min(32, (pieces - k0 + parts - 1) / parts);
       float2 u = make_float2(-INFINITY, 0.f);
       if (lane < here) u = __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot_row(k0 + lane * parts, row) * 2));
       float w = 0.f;
-      for (int i0 = 0; i0 < here; i0 += 8) {
-        float y[8][V];
+      for (int i0 = 0; i0 < here; i0 += 16) {
+        float y[16][V];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 16; ++i) {
           const float* src = p.part_o + slot_row(k0 + min(i0 + i, here - 1) * parts, row) * D + lane * V;
           if (V == 4)
             *reinterpret_cast<float4*>(y[i]) = __ldcg(reinterpret_cast<const float4*>(src));
@@ -364,7 +364,7 @@ __device__ __forceinline__ void join(const FewParams& p, float* red, int first_b
           l += u.y * w;
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 16; ++i) {
           const float f = __shfl_sync(0xffffffffu, w, i0 + i);
           if (i0 + i < here) {
 #pragma unroll
@@ -402,7 +402,7 @@ __device__ __forceinline__ void join(const FewParams& p, float* red, int first_b
     }
     if (there && part == 0) {
       const float inv = m == -INFINITY ? 0.f : vf / l;
-      const int t = (row0 + row) / a.group, g = (row0 + row) % a.group;
+      const int t = a.token_of(row0 + row), g = row0 + row - t * a.group;
       uint16_t* dst = a.o + (first + t) * a.o_stride_t + (static_cast<long long>(head) * a.group + g) * a.o_stride_h +
                       lane * V;
 #pragma unroll
@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
     const int head = unit % a.kv_heads;
     const int row0 = unit / a.kv_heads * C::ROWS;
     const int nrows = min(C::ROWS, sh.rows - row0);
-    const int len = sh.len, tokens = sh.rows / a.group;
+    const int len = sh.len, tokens = a.token_of(sh.rows);
     const int k_begin = max(off, 1) - 1, k_end = stop - 1;  // steps that hold keys
     const int* table = a.tables + static_cast<long long>(r) * a.width;
     const bool starts = off == 0, ends = stop == sh.steps;
@@ -528,6 +528,20 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
     // the unit's count is looked at here, and set up long before it is needed
     unsigned long long count_was = p.epoch << 16;
     if (!(starts && ends) && threadIdx.x == 0) count_was = *reinterpret_cast<volatile unsigned long long*>(count);
+
+    // ---- query rows, 16 bytes per thread and turn: loads first
+    constexpr int PER_ROW = D / 8, Q_TURNS = (C::ROWS * PER_ROW + THREADS - 1) / THREADS;
+    uint4 q[Q_TURNS];
+#pragma unroll
+    for (int i = 0; i < Q_TURNS; ++i) {
+      const int at = i * THREADS + threadIdx.x, row = at / PER_ROW, ch = at % PER_ROW;
+      q[i] = make_uint4(0, 0, 0, 0);
+      if (row < nrows) {
+        const int t = a.token_of(row0 + row), g = row0 + row - t * a.group;
+        q[i] = *reinterpret_cast<const uint4*>(a.q + (sh.first + t) * a.q_stride_t +
+                                               (static_cast<long long>(head) * a.group + g) * a.q_stride_h + ch * 8);
+      }
+    }
 
     // ---- copies of this warp's first steps
     int page_ids = 0, ids_at = -32;  // page of step k_begin + warp + WARPS * (ids_at + lane)
@@ -561,19 +575,13 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
 #pragma unroll
     for (int i = 0; i < C::STAGES - 1; ++i) issue();
 
-    // ---- query rows, 16 bytes per thread and turn, in the order of the B fragments
-    constexpr int PER_ROW = D / 8;
+    // ---- query rows into the order of the B fragments
 #pragma unroll
-    for (int i = 0; i < C::ROWS * PER_ROW; i += THREADS) {
-      const int at = i + threadIdx.x;
+    for (int i = 0; i < Q_TURNS; ++i) {
+      const int at = i * THREADS + threadIdx.x;
       if (C::ROWS * PER_ROW % THREADS == 0 || at < C::ROWS * PER_ROW) {
         const int row = at / PER_ROW, ch = at % PER_ROW;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (row < nrows) {
-          const int t = (row0 + row) / a.group, g = (row0 + row) % a.group;
-          x = *reinterpret_cast<const uint4*>(a.q + (sh.first + t) * a.q_stride_t +
-                                              (static_cast<long long>(head) * a.group + g) * a.q_stride_h + ch * 8);
-        }
+        uint4 x = q[i];
         float f = 1.f;
         if (BF16) {
           // bf16 rows are scaled by a power of two that brings their largest
@@ -619,11 +627,11 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
       for (int i = 0; i < 2; ++i) {
         const int row = nt * 8 + 2 * c + i;
         factor[nt][i] = kf * rowf[row];
-        limit[nt][i] = a.causal && row < nrows ? len - tokens + 1 + (row0 + row) / a.group : len;
+        limit[nt][i] = a.causal && row < nrows ? len - tokens + 1 + a.token_of(row0 + row) : len;
         acc.m[nt][i] = -INFINITY;
         acc.l[nt][i] = 0.f;
       }
-    least = a.causal ? min(len, len - tokens + 1 + row0 / a.group) : len;
+    least = a.causal ? min(len, len - tokens + 1 + a.token_of(row0)) : len;
 #pragma unroll
     for (int t = 0; t < D / 16; ++t)
 #pragma unroll
@@ -698,7 +706,7 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
       }
       if (starts && ends) {
         const float inv = m == -INFINITY ? 0.f : vf / l;
-        const int t = (row0 + row) / a.group, g = (row0 + row) % a.group;
+        const int t = a.token_of(row0 + row), g = row0 + row - t * a.group;
         store4<BF16>(a.o + (sh.first + t) * a.o_stride_t +
                          (static_cast<long long>(head) * a.group + g) * a.o_stride_h + d,
                      make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
@@ -754,7 +762,7 @@ struct Plan {
   int blocks;
   size_t ml_off, done_off, many_off, bytes;
   bool fits;
-  ManyPlan many;  // max_blocks 0: no request has that many rows
+  ManyPlan many;  // max_units 0: no request has that many rows
 };
 static Plan plan_of(const gfx906_b200_cache4_attn_args& g, int sms) {
   Plan pl{};
@@ -802,22 +810,27 @@ static int attn(const gfx906_b200_cache4_attn_args& g, void* ws, size_t ws_bytes
   const int rc = gfx906_b200_internal_device(&sms);
   if (rc != GFX906_B200_OK) return rc;
   const Plan pl = plan_of(g, sms);
-  if (!pl.fits || (static_cast<long long>(g.max_tokens) * (g.heads / g.kv_heads) > FEW_ROWS && !pl.many.max_blocks) || !ws || ws_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(ws) & 255u)) return GFX906_B200_EINVAL;
+  if (!pl.fits || (static_cast<long long>(g.max_tokens) * (g.heads / g.kv_heads) > FEW_ROWS && !pl.many.max_units) || !ws || ws_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(ws) & 255u)) return GFX906_B200_EINVAL;
   FewParams p{};
   p.a = {static_cast<const uint16_t*>(g.q), static_cast<uint16_t*>(g.o), static_cast<const uint8_t*>(g.cache), g.tables,
          g.lengths, g.query_start, g.k_scale, g.v_scale, g.q_stride_t, g.q_stride_h, g.o_stride_t, g.o_stride_h,
          g.tokens, g.kv_heads, g.heads / g.kv_heads, g.pages, g.requests, g.width, g.causal != 0, g.zero_rest != 0,
-         g.scale * 1.4426950408889634f};
+         g.scale * 1.4426950408889634f,
+         group_magic(static_cast<long long>(g.tokens) * (g.heads / g.kv_heads), g.heads / g.kv_heads)};
   p.max_rows = INT_MAX;
   uint8_t* base = static_cast<uint8_t*>(ws);
-  if (pl.many.max_blocks > 0) {
+  if (pl.many.max_units > 0) {
     ManyParams m{};
     m.a = p.a;
     m.min_rows = p.max_rows = FEW_ROWS;
-    m.max_blocks = pl.many.max_blocks;
-    m.pieces = pl.many.pieces;
+    m.max_units = pl.many.max_units;
+    m.sms = sms;
+    m.max_units = pl.many.max_units;
+    m.sms = sms;
     m.part_o = reinterpret_cast<float*>(base + pl.many_off);
     m.part_ml = reinterpret_cast<float*>(base + pl.many_off + pl.many.ml_off);
+    m.done = reinterpret_cast<unsigned long long*>(base + pl.many_off + pl.many.done_off);
+    m.epoch = gfx906_b200_internal_next_epoch() & 0xffffffffffffull;
     m.timeout_ns = gfx906_b200_internal_timeout_ns();
     const int st = launch_many(m, g.D, g.dtype, stream);
     if (st != GFX906_B200_OK) return st;

@@ -18,7 +18,18 @@ struct AttnParams {
   int tokens, kv_heads, group, pages, requests, width;
   int causal, zero_rest;
   float scale_log2;  // scale * log2(e)
+  unsigned group_magic;  // ceil(2^32 / group) where rows / group is its high product, else 0
+
+  // Of query row `row` of a request (token * group + head of the group): its token.
+  __device__ __forceinline__ int token_of(int row) const {
+    return group_magic ? static_cast<int>(__umulhi(static_cast<unsigned>(row), group_magic)) : row / group;
+  }
 };
+
+// The product's error is below row * group / 2^32 of a token.
+inline unsigned group_magic(long long rows, int group) {
+  return group > 1 && rows * group < (1ll << 32) ? static_cast<unsigned>(((1ll << 32) + group - 1) / group) : 0u;
+}
 
 // Query rows of request r: first token and number of tokens, whatever the
 // array holds (it comes from the caller's device memory).

@@ -14,15 +14,20 @@
 // row's maximum, sum, exponentials and output scaling); 8-11 the conversion; 12
 // issues the products.
 //
-// When a call has fewer units than half the SMs, each unit's keys are cut into
-// `pieces` runs with a CTA each; their partial sums (32 bits, in the workspace)
-// are joined by cache4_many_join_kernel.
+// Units are dealt to the SMs as these become free, those with the most keys
+// first. The units of the last, partial wave (all of them, if they are fewer
+// than the SMs) are cut into pieces of their key range, whose partial sums
+// (32 bits, in the workspace) the CTA that finishes the last piece joins.
 //
 // Every wait is bounded (time limit from the host), as in the dense kernels: one
 // that runs out sets the device status word and the CTA ends.
 #include <limits.h>
 #include <math.h>
 
+// All exponentials on MUFU here, none by polynomial: the conversions already
+// keep the FMA pipe busy (4096 rows x 24 heads against 16384 keys: 775 us; with
+// one pair in four on the FMA pipe, as the dense kernels have it, 793; two, 899).
+#define ATTN_EMU_PAIRS 0
 #include "attn_row.cuh"
 #include "cache4.cuh"
 #include "cache4_attn.cuh"
@@ -39,10 +44,13 @@ constexpr int M_THREADS = 512;
 constexpr int CONVERT_WARP = 8;      // four of them
 constexpr int ISSUE_WARP = 12;
 constexpr int BOX = 16384;           // 128 rows x 64 fp16 columns, 128-byte swizzle
-// Registers: 512 threads at 128 each are launched; 256 * 192 + 128 * 96 + 128 * 32 = 65536.
-constexpr uint32_t M_REGS_SOFTMAX = 192;
-constexpr uint32_t M_REGS_CONVERT = 96;
-constexpr uint32_t M_REGS_ISSUE = 32;
+// Registers: 512 threads at 128 each are launched; 256 * 184 + 128 * 64 + 128 * 80
+// = 65536. The issue loop is on the critical path of every tile: with 32
+// registers instead of 80 the compiler spilled in it, and 4096 rows x 24 heads
+// against 16384 keys took 1086 us instead of 809 (48: 959, 72: 913).
+constexpr uint32_t M_REGS_SOFTMAX = 184;
+constexpr uint32_t M_REGS_CONVERT = 64;
+constexpr uint32_t M_REGS_ISSUE = 80;
 constexpr float M_RESCALE = 8.0f;    // log2 units, see the dense kernels
 constexpr float M_LARGE = 67108864.f;  // 2^26: half a 32-bit step is 2 log2 units
 
@@ -57,26 +65,33 @@ struct Many {
   static constexpr int B_K_FULL = 1, B_K_EMPTY = B_K_FULL + SLOTS;
   static constexpr int B_V_FULL = B_K_EMPTY + SLOTS, B_V_EMPTY = B_V_FULL + SLOTS;
   static constexpr int B_S = B_V_EMPTY + SLOTS, B_P_HALF = B_S + 2, B_P = B_P_HALF + 2, B_O = B_P + 2;
-  static constexpr int B_DRAIN = B_O + 2;
+  static constexpr int B_WG = B_O + 2;  // [2] rendezvous of a softmax warpgroup
+  static constexpr int B_DRAIN = B_WG + 2;
   static constexpr int BARS = B_DRAIN + 1;
   static constexpr int K_OFF = 2 * TILE, V_OFF = K_OFF + SLOTS * TILE, BAR_OFF = V_OFF + SLOTS * TILE;
-  static constexpr int STAGE_OFF = (BAR_OFF + BARS * 8 + 16 + 127) & ~127;  // 4 KiB per softmax warp
+  static constexpr int ROWF_OFF = BAR_OFF + BARS * 8 + 16;  // [2][128] exponents of Q's rows, a byte each
+  static constexpr int STAGE_OFF = (ROWF_OFF + 2 * M_ROWS + 127) & ~127;  // 4 KiB per softmax warp
   static constexpr int SMEM = 1024 + STAGE_OFF + 8 * 4096;
   static_assert(SMEM <= 232448, "");
 };
 
+// Bounded waits for the barriers at `bars`; the word at `abort_at` stops all of them.
 struct Waiter {
-  uint32_t bars;
-  volatile int* abort_flag;
-  unsigned long long timeout_ns;
+  uint32_t bars, abort_at;
+  const ManyParams& p;
+  __device__ __forceinline__ int aborted() const {
+    int v;
+    asm volatile("ld.volatile.shared.s32 %0, [%1];" : "=r"(v) : "r"(abort_at) : "memory");
+    return v;
+  }
   __device__ __forceinline__ bool slow(uint32_t bar, uint32_t parity, bool heed_abort) const {
     const uint64_t t0 = globaltimer_ns();
     uint32_t n = 0;
     while (true) {
       if (mbar_try_wait(bar, parity)) return true;
-      if (heed_abort && *abort_flag) return false;
-      if ((++n & 31u) == 0u && (globaltimer_ns() - t0 > (heed_abort ? timeout_ns : 100000000ull) || n > (1u << 24))) {
-        *abort_flag = 1;
+      if (heed_abort && aborted()) return false;
+      if ((++n & 31u) == 0u && (globaltimer_ns() - t0 > (heed_abort ? p.timeout_ns : 100000000ull) || n > (1u << 24))) {
+        asm volatile("st.volatile.shared.s32 [%0], %1;" ::"r"(abort_at), "r"(1) : "memory");
         atomicOr(&g_cache4_status, 1u);
         return false;
       }
@@ -85,7 +100,8 @@ struct Waiter {
   // Every lane of the warp gets the same answer.
   __device__ __forceinline__ bool operator()(int idx, uint32_t parity) const {
     const uint32_t bar = bars + 8u * idx;
-    const bool ok = mbar_try_wait(bar, parity) || slow(bar, parity, true);
+    bool ok = mbar_try_wait(bar, parity);
+    if (!ok) ok = slow(bar, parity, true);
     return __all_sync(0xffffffffu, ok);
   }
 };
@@ -204,24 +220,72 @@ __device__ __forceinline__ void put_v(Codes<D>& r, uint32_t tile, int row0, int 
   }
 }
 
-// The unit of CTA `index` of the launch: request, its first block's index among
-// all blocks, and the block wanted; false: no such unit.
-struct Unit {
-  int r, block;  // request, block of 256 rows within it
+// What a CTA does: a unit (a block of 256 rows of a request, and a kv head), and
+// which of the pieces of its key range.
+struct Work {
+  int r, block, head;   // r < 0: nothing
+  int piece, most;      // piece of at most `most`
+  int tail;             // number of the unit among those that are cut
+};
+// The same with what follows from it, in shared memory.
+struct Seg {
+  int r, head, row0;     // request, kv head, first of its query rows
+  int first, n, len;     // of the request
+  int t0, t1;            // tiles of 128 keys
+  int tail, piece, pieces;
 };
 __device__ __forceinline__ int many_blocks(const ManyParams& p, int r) {
-  const long long rows = static_cast<long long>(rows_of(p.a, r).n) * p.a.group;
-  return rows > p.min_rows ? static_cast<int>((rows + 2 * M_ROWS - 1) / (2 * M_ROWS)) : 0;
+  const Rows t = rows_of(p.a, r);
+  const int rows = t.n * p.a.group;
+  return rows > p.min_rows ? (rows + 2 * M_ROWS - 1) / (2 * M_ROWS) : 0;
 }
-// Whole block of THREADS threads.
-template <int THREADS>
-__device__ __forceinline__ bool find_unit(const ManyParams& p, int want, Unit* out) {
-  __shared__ int part[THREADS / 32];
+constexpr int MAX_PIECES = 16;
+constexpr int CUT_CTAS = 3;   // times the SMs: pieces of all units that are cut, at most
+constexpr int MIN_TILES = 4;  // of 128 keys, in a piece
+
+// All threads of the CTA. Units are numbered from the last block of the last
+// request down, the kv heads of a block one after the other: of one request,
+// the blocks that see the most keys come first.
+__device__ __forceinline__ Work find_work(const ManyParams& p) {
+  __shared__ int part[M_THREADS / 32];
   __shared__ int found[2];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  int total = 0;
-  if (threadIdx.x == 0) found[0] = -1;
-  for (int base = 0; base < p.a.requests && total <= want; base += THREADS) {
+  long long blocks = 0;
+  for (int base = 0; base < p.a.requests; base += M_THREADS) {
+    const int r = base + threadIdx.x;
+    const int w = __reduce_add_sync(0xffffffffu, r < p.a.requests ? many_blocks(p, r) : 0);
+    if (lane == 0) part[warp] = w;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < M_THREADS / 32; ++i) blocks += part[i];
+    __syncthreads();
+  }
+  Work out{-1, 0, 0, 0, 1, 0};
+  if (blocks > p.max_units / p.a.kv_heads) return out;  // query_start decreases somewhere
+  const int units = static_cast<int>(blocks) * p.a.kv_heads;
+  const int tail = units % p.sms, whole = units - tail;
+  // the number of pieces that ends the last wave soonest (a lane tries each),
+  // with a hundredth of a unit as the price of a piece
+  const int pieces = lane % MAX_PIECES + 1;
+  const int cost = pieces == 1 || tail * pieces <= CUT_CTAS * p.sms
+                       ? (tail * pieces + p.sms - 1) / p.sms * 1000 / pieces + 10 * pieces
+                       : 1 << 20;
+  out.most = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<unsigned>(cost) * MAX_PIECES + pieces - 1) %
+                              MAX_PIECES) + 1;
+  int unit = blockIdx.x;
+  if (unit >= whole) {
+    const int i = unit - whole;
+    out.tail = i / out.most;
+    out.piece = i % out.most;
+    unit = whole + out.tail;
+  } else {
+    out.most = 1;
+  }
+  if (unit >= units) return out;
+  out.head = unit % p.a.kv_heads;
+  const int want = static_cast<int>(blocks) - 1 - unit / p.a.kv_heads;
+  int before = 0;
+  for (int base = 0; base < p.a.requests && before <= want; base += M_THREADS) {
     const int r = base + threadIdx.x;
     const int w = r < p.a.requests ? many_blocks(p, r) : 0;
     int inc = w;
@@ -232,22 +296,140 @@ __device__ __forceinline__ bool find_unit(const ManyParams& p, int want, Unit* o
     }
     if (lane == 31) part[warp] = inc;
     __syncthreads();
-    int before = total + inc - w;
+    int mine = before + inc - w;
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) {
-      if (i < warp) before += part[i];
-      total += part[i];
+    for (int i = 0; i < M_THREADS / 32; ++i) {
+      if (i < warp) mine += part[i];
+      before += part[i];
     }
-    if (before <= want && want < before + w) {
+    if (mine <= want && want < mine + w) {
       found[0] = r;
-      found[1] = want - before;
+      found[1] = want - mine;
     }
     __syncthreads();
   }
-  __syncthreads();
-  out->r = found[0];
-  out->block = found[1];
-  return found[0] >= 0;
+  out.r = found[0];
+  out.block = found[1];
+  return out;
+}
+
+// One row of the pieces of a unit, added in their order.
+template <int D, bool BF16>
+__device__ __forceinline__ void join_row(const ManyParams& p, int tail, int pieces, int row, int head, uint16_t* out) {
+  const long long slot0 = static_cast<long long>(tail) * MAX_PIECES;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot0 * 2 * M_ROWS + row;
+  float m = -INFINITY, l = 0.f;
+  for (int k = 0; k < pieces; ++k) m = fmaxf(m, __ldcg(ml + k * 2 * M_ROWS).x);
+  for (int k = 0; k < pieces; ++k) {
+    const float2 u = __ldcg(ml + k * 2 * M_ROWS);
+    l += u.x == -INFINITY ? 0.f : u.y * ex2_approx(u.x - m);
+  }
+  const float inv = m == -INFINITY ? 0.f : (p.a.v_scale ? p.a.v_scale[head] : 1.f) / l;
+#pragma unroll 1
+  for (int c = 0; c < D; c += 32) {
+    float x[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) x[e] = 0.f;
+#pragma unroll 2
+    for (int k = 0; k < pieces; ++k) {
+      const float mk = __ldcg(ml + k * 2 * M_ROWS).x;
+      const float f = mk == -INFINITY ? 0.f : ex2_approx(mk - m);
+      const float4* src = reinterpret_cast<const float4*>(p.part_o + (slot0 + k) * 2 * M_ROWS * D) + row;
+      float4 y[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) y[q] = __ldcg(src + (c / 4 + q) * 2 * M_ROWS);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        x[4 * q] += y[q].x * f;
+        x[4 * q + 1] += y[q].y * f;
+        x[4 * q + 2] += y[q].z * f;
+        x[4 * q + 3] += y[q].w * f;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t h[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = float2_to_pair<BF16>(x[8 * q + 2 * e] * inv, x[8 * q + 2 * e + 1] * inv);
+      *reinterpret_cast<uint4*>(out + c + 8 * q) = make_uint4(h[0], h[1], h[2], h[3]);
+    }
+  }
+}
+
+// A warp's 32 rows of a query tile, from row0 on, into the swizzled layout of the
+// tensor core's A operand, whole rows per D / 8 lanes; rows behind the request's
+// last are zero. Rows of bf16 are
+// divided by a power of two that brings their largest number to [1, 2) and then
+// fit fp16 (what falls below 2^-24 of a row's largest is lost); rowf[row] keeps
+// its exponent.
+template <int D, bool BF16>
+__device__ __forceinline__ void put_q(const AttnParams& a, const Seg& sg, int tile0, int row0, int lane, uint32_t tile,
+                                      uint8_t* rowf) {
+  constexpr int LANES = D / 8, ROWS = 32 / LANES;  // lanes of a row, rows of an access
+  const int total = sg.n * a.group, ch = lane % LANES;
+  const uint16_t* q = a.q + sg.first * a.q_stride_t + static_cast<long long>(sg.head) * a.group * a.q_stride_h + ch * 8;
+  auto place = [&](int row) { return tile + (ch / 8) * BOX + row * 128 + (((ch % 8) ^ (row & 7)) << 4); };
+#pragma unroll 8
+  for (int row = row0 + lane / LANES; row < row0 + 32; row += ROWS) {
+    const int at = tile0 + row, t = a.token_of(at);
+    const bool there = at < total;
+    const uint16_t* src = there ? q + t * a.q_stride_t + (at - t * a.group) * a.q_stride_h : a.q;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place(row)), "l"(src), "r"(there ? 16 : 0)
+                 : "memory");
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (BF16) {  // each lane finds what it fetched itself
+#pragma unroll 4
+    for (int row = row0 + lane / LANES; row < row0 + 32; row += ROWS) {
+      const uint4 x = ld_shared_v4(place(row));
+      uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      float mx = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = bf162_to_float2(w[e]);
+        mx = fmax3(mx, fabsf(f.x), fabsf(f.y));
+      }
+#pragma unroll
+      for (int d = LANES / 2; d > 0; d /= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+      const uint32_t ex = (__float_as_uint(mx) >> 23) & 255u;
+      const bool scaled = ex > 0 && ex < 254;
+      const float inv = scaled ? __uint_as_float((254u - ex) << 23) : 1.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = bf162_to_float2(w[e]);
+        w[e] = pack_half2(f.x * inv, f.y * inv);
+      }
+      if (ch == 0) rowf[row] = static_cast<uint8_t>(scaled ? ex : 127u);
+      st_shared_v4(place(row), w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// The thread's number, read anew: nothing that follows from it is kept meanwhile.
+__device__ __forceinline__ int fresh_tid() {
+  int t;
+  asm volatile("mov.u32 %0, %%tid.x;" : "=r"(t));
+  return t;
+}
+__device__ __forceinline__ int tile_of() { return fresh_tid() / M_ROWS; }
+// Where a softmax thread is in a unit.
+struct Place {
+  int tile, row, total, tile0, my_row;  // query tile, row in it; rows of the request, the tile's first, this one
+  bool live;
+  __device__ __forceinline__ Place(const Seg& s, const AttnParams& a) {
+    const int t = fresh_tid();
+    tile = t / M_ROWS;
+    row = t % M_ROWS;
+    total = s.n * a.group;
+    tile0 = s.row0 + tile * M_ROWS;
+    my_row = tile0 + row;
+    live = my_row < total;
+  }
+};
+// Is page i of the unit's request, as far as it holds tokens, outside the cache?
+__device__ __forceinline__ bool page_missing(const AttnParams& a, const Seg& s, int i) {
+  return i * PAGE < s.len &&
+         static_cast<unsigned>(__ldg(a.tables + static_cast<long long>(s.r) * a.width + i)) >= static_cast<unsigned>(a.pages);
 }
 
 template <int D, bool BF16>
@@ -260,24 +442,27 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
   griddep_wait();
   if (threadIdx.x == 0) griddep_launch_dependents();
 
-  // the last blocks of a request see the most keys: they come first
-  const int per_block = a.kv_heads * p.pieces;
-  const int head = static_cast<int>(blockIdx.x) % per_block / p.pieces;
-  const int piece = static_cast<int>(blockIdx.x) % p.pieces;
-  const int want = p.max_blocks - 1 - static_cast<int>(blockIdx.x) / per_block;
-  Unit u;
-  if (!find_unit<M_THREADS>(p, want, &u)) return;
-  const Rows rows = rows_of(a, u.r);
-  const int len = length_of(a, u.r);
-  const int row0 = u.block * 2 * M_ROWS;
-  const int total_rows = rows.n * a.group;
-  const bool has1 = row0 + M_ROWS < total_rows;
-  const int last_token = (min(total_rows, row0 + 2 * M_ROWS) - 1) / a.group;
-  const int seen = a.causal ? max(0, min(len, len - rows.n + 1 + last_token)) : len;
-  const int all_tiles = (seen + BN - 1) / BN;
-  const int t0 = static_cast<int>(static_cast<long long>(all_tiles) * piece / p.pieces);
-  const int t1 = static_cast<int>(static_cast<long long>(all_tiles) * (piece + 1) / p.pieces);
-  const int* table = a.tables + static_cast<long long>(u.r) * a.width;
+  __shared__ Seg sg;
+  {
+    const Work u = find_work(p);
+    if (u.r < 0) return;
+    const Rows rows = rows_of(a, u.r);
+    const int len = length_of(a, u.r), row0 = u.block * 2 * M_ROWS;
+    const int last_token = a.token_of(min(rows.n * a.group, row0 + 2 * M_ROWS) - 1);
+    const int seen = a.causal ? max(0, min(len, len - rows.n + 1 + last_token)) : len;
+    const int tiles = (seen + BN - 1) / BN;
+    const int pieces = max(1, min(u.most, tiles / MIN_TILES));
+    if (u.piece >= pieces) return;
+    if (threadIdx.x == 0) {
+      sg = {u.r, u.head, row0, rows.first, rows.n, len, tiles * u.piece / pieces, tiles * (u.piece + 1) / pieces,
+            u.tail, u.piece, pieces};
+      for (int i = 0; i < 2 && pieces > 1; ++i) {  // set up the unit's counts, long before they are needed
+        unsigned long long* count = p.done + u.tail * 2 + i;
+        const unsigned long long was = *reinterpret_cast<volatile unsigned long long*>(count);
+        if ((was >> 16) != p.epoch) atomicCAS(count, was, p.epoch << 16);
+      }
+    }
+  }
 
   const uint32_t raw = smem_u32(many_smem);
   const uint32_t s0 = (raw + 1023u) & ~1023u;
@@ -285,8 +470,9 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
   const uint32_t bars = s0 + C::BAR_OFF;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::BAR_OFF + C::BARS * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* last_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);  // [2], per tile
   if (threadIdx.x == 0) {
-    mbar_init(bars + 8 * C::B_Q, 2 * M_ROWS);
+    mbar_init(bars + 8 * C::B_Q, sg.row0 + M_ROWS < sg.n * a.group ? 2 * M_ROWS : M_ROWS);
     for (int s = 0; s < C::SLOTS; ++s) {
       mbar_init(bars + 8 * (C::B_K_FULL + s), 4);
       mbar_init(bars + 8 * (C::B_K_EMPTY + s), 1);
@@ -298,6 +484,8 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
       mbar_init(bars + 8 * (C::B_P_HALF + i), M_ROWS);
       mbar_init(bars + 8 * (C::B_P + i), M_ROWS);
       mbar_init(bars + 8 * (C::B_O + i), 1);
+      mbar_init(bars + 8 * (C::B_WG + i), M_ROWS);
+      last_flag[i] = 0;
     }
     mbar_init(bars + 8 * C::B_DRAIN, 1);
     *abort_flag = 0;
@@ -312,11 +500,13 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const Waiter wait{bars, abort_flag, p.timeout_ns};
+  const Waiter wait{bars, smem_u32(tmem_slot + 1), p};
 
   if (warp >= ISSUE_WARP) {
     // ------------------------------------------------------ issue of products
     setmaxnreg_dec<M_REGS_ISSUE>();
+    const int t0 = sg.t0, t1 = sg.t1;
+    const bool has1 = sg.row0 + M_ROWS < sg.n * a.group;
     if (warp == ISSUE_WARP && t0 < t1) {
       constexpr uint32_t IDESC_QK = idesc_f16_f32(M_ROWS, BN, 0, 0);
       constexpr uint32_t IDESC_PV = idesc_f16_f32(M_ROWS, D, 0, 1);
@@ -386,7 +576,9 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
     // ------------------------------------------------------------- conversion
     setmaxnreg_dec<M_REGS_CONVERT>();
     const int w = warp - CONVERT_WARP;  // blocks w and w + 4 of a tile: one in each of its pages
-    const uint8_t* cache = a.cache + static_cast<long long>(head) * L::PAGE_BYTES + w * L::BLOCK_BYTES;
+    const int len = sg.len, t0 = sg.t0, t1 = sg.t1;
+    const int* table = a.tables + static_cast<long long>(sg.r) * a.width;
+    const uint8_t* cache = a.cache + static_cast<long long>(sg.head) * L::PAGE_BYTES + w * L::BLOCK_BYTES;
     const long long page_stride = static_cast<long long>(a.kv_heads) * L::PAGE_BYTES;
     const int pages_held = (len + PAGE - 1) / PAGE;
     // where this warp's block of page 2 j + i is, or null
@@ -430,73 +622,43 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
     }
   } else {
     // ---------------------------------------------------------------- softmax
+    // A score row fills 128 registers, and what else lives through the loop over
+    // the tiles decides whether the compiler has to spill it (measured: 1.5
+    // times the time). So that is kept to what each tile needs -- the flags
+    // are bits of one word -- and everything else is
+    // looked up again behind the loop, from the thread's number and the unit.
     setmaxnreg_inc<M_REGS_SOFTMAX>();
-    const int ti = warp >> 2, quad = warp & 3;
-    const int row = quad * 32 + lane;
-    const int my_row = row0 + ti * M_ROWS + row;  // of the request
-    const bool live = my_row < total_rows;
-    float factor = 1.f;
-    if (ti == 0 || has1) {
-      // this thread's row of q, in the swizzled layout of the tensor core's A operand
-      const int t = my_row / a.group, g = my_row % a.group;
-      const uint4* src = reinterpret_cast<const uint4*>(
-          a.q + (rows.first + t) * a.q_stride_t + (static_cast<long long>(head) * a.group + g) * a.q_stride_h);
-      uint4 x[D / 8];
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) x[c] = live ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-      if (BF16) {
-        // rows of bf16 are brought to [1, 2) by a power of two and then fit fp16
-        // (what falls below 2^-24 of a row's largest is lost)
-        float mx = 0.f;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = bf162_to_float2(w[e]);
-            mx = fmax3(mx, fabsf(f.x), fabsf(f.y));
-          }
-        }
-        const uint32_t ex = (__float_as_uint(mx) >> 23) & 255u;
-        const bool scaled = ex > 0 && ex < 254;
-        if (scaled) factor = __uint_as_float(ex << 23);
-        const float inv = scaled ? __uint_as_float((254u - ex) << 23) : 1.f;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = bf162_to_float2(w[e]);
-            w[e] = pack_half2(f.x * inv, f.y * inv);
-          }
-          x[c] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+    enum : uint32_t { S_PARITY = 1, LARGE = 2, HOLES = 4, FIRST = 8, OK = 16 };
+    const uint32_t bar = bars + 8 * (warp >> 2);  // of this query tile: index + tile
+    const uint32_t tS = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + (warp >> 2) * 128;
+    uint32_t st = OK;
+    auto tile_wait = [&](int idx, uint32_t parity) -> bool {
+      bool ok = mbar_try_wait(bar + 8u * idx, parity);
+      if (!ok) ok = wait.slow(bar + 8u * idx, parity, true);
+      return __all_sync(0xffffffffu, ok);
+    };
+    if (sg.row0 + (warp >> 2) * M_ROWS < sg.n * a.group) {
+      float sl2 = a.scale_log2 * (a.k_scale ? a.k_scale[sg.head] : 1.f);
+      int left = sg.t1 - sg.t0;  // tiles
+      int until;                 // keys that this row sees from the next tile's first on
+      {
+        const Place at(sg, a);
+        put_q<D, BF16>(a, sg, at.tile0, at.row - lane, lane, s0 + at.tile * C::TILE, smem + C::ROWF_OFF + at.tile * M_ROWS);
+        fence_proxy_async_smem();
+        mbar_arrive(bars + 8 * C::B_Q);
+        __syncwarp();
+        if (BF16) sl2 *= __uint_as_float(static_cast<uint32_t>(smem[C::ROWF_OFF + threadIdx.x]) << 23);
+        until = (a.causal && at.live ? min(sg.len, sg.len - sg.n + 1 + a.token_of(at.my_row)) : sg.len) - sg.t0 * BN;
+        bool holes = false;
+        for (int i = 2 * sg.t0 + lane; i < 2 * sg.t1; i += 32) holes |= page_missing(a, sg, i);
+        if (__any_sync(0xffffffffu, holes)) st |= HOLES;
       }
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c)
-        st_shared_v4(s0 + ti * C::TILE + (c / 8) * BOX + row * 128 + (((c % 8) ^ (row & 7)) << 4), x[c].x, x[c].y,
-                     x[c].z, x[c].w);
-    }
-    fence_proxy_async_smem();
-    mbar_arrive(bars + 8 * C::B_Q);
-
-    if (ti == 0 || has1) {
-      const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
-      const uint32_t tS = tmem + lane_off + ti * 128;
-      const uint32_t tO = tmem + lane_off + 256 + ti * D;
-      const float sl2 = a.scale_log2 * (a.k_scale ? a.k_scale[head] : 1.f) * factor;
-      const bool pos = sl2 >= 0.f;
-      // keys this row sees: [0, limit)
-      const int limit = a.causal && live ? min(len, len - rows.n + 1 + my_row / a.group) : len;
-      bool holes = false;  // pages outside the cache, whose keys take no part
-      for (int i = 2 * t0 + lane; i < 2 * t1 && i * PAGE < len; i += 32)
-        holes |= static_cast<unsigned>(__ldg(table + i)) >= static_cast<unsigned>(a.pages);
-      holes = __any_sync(0xffffffffu, holes);
       float m = -INFINITY, l = 0.f;
-      bool ok = true, large = false;
-      for (int j = t0; j < t1; ++j) {
-        const uint32_t parity = (j - t0) & 1;
-        if (!wait(C::B_S + ti, parity)) { ok = false; break; }
+      st |= FIRST;
+#pragma unroll 1
+      for (; left > 0; --left, until -= BN) {
+        if (!tile_wait(C::B_S, st & S_PARITY)) { st &= ~OK; break; }
+        st ^= S_PARITY;
         tc_fence_after();
         uint32_t s[BN];
 #pragma unroll
@@ -504,114 +666,130 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
         tmem_wait_ld();
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) reg_fence32(s + 32 * c);
-        int lo = 0, hi = min(BN, limit - j * BN);
-        if (holes) {
-          const bool h0 = static_cast<unsigned>(__ldg(table + 2 * j)) >= static_cast<unsigned>(a.pages);
-          const bool h1 = (2 * j + 1) * PAGE < len &&
-                          static_cast<unsigned>(__ldg(table + 2 * j + 1)) >= static_cast<unsigned>(a.pages);
-          if (h0) lo = PAGE;
-          if (h1) hi = min(hi, PAGE);
+        int lo = 0, hi = min(BN, until);
+        if (st & HOLES) {  // pages outside the cache, whose keys take no part
+          const int j = sg.t1 - left;
+          if (page_missing(a, sg, 2 * j)) lo = PAGE;
+          if (page_missing(a, sg, 2 * j + 1)) hi = min(hi, PAGE);
         }
         const bool full = __all_sync(0xffffffffu, lo == 0 && hi == BN);
-        const float mx = row_extreme(s, hi, full, pos, lo);
-        const float m_cand = lo < hi ? mx * sl2 : -INFINITY;
-        const float m_new = fmaxf(m, m_cand);
+        const float mx = row_extreme(s, hi, full, sl2 >= 0.f, lo);
+        const float m_new = lo < hi ? fmaxf(m, mx * sl2) : m;
         const bool need = m_new > m + M_RESCALE;
-        float f = 1.f;
-        if (need) {
-          f = ex2_approx(m - m_new);
-          m = m_new;
-        }
         if (__any_sync(0xffffffffu, need)) {
-          rescale_rows<D>(tO, j > t0, f);
+          float f = 1.f;
+          if (need) {
+            f = ex2_approx(m - m_new);
+            m = m_new;
+          }
+          rescale_rows<D>(tS + 256 - (D == 128 ? 0 : (tile_of() * (128 - D))), !(st & FIRST), f);
           l *= f;
-          large = __any_sync(0xffffffffu, fabsf(m) > M_LARGE && m > -INFINITY);
+          if (__any_sync(0xffffffffu, fabsf(m) > M_LARGE && m > -INFINITY)) st |= LARGE;
         }
-        float neg_m = m == -INFINITY ? 0.f : -m, mul = sl2;
-        if (large) {
-          // Scores so large that m is a rounded product: round each score as m
-          // was, or the largest would lie half a step of m above or below it.
-#pragma unroll
-          for (int c = 0; c < BN; ++c)
-            s[c] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(s[c]), sl2), neg_m));
-          mul = 1.f;
-          neg_m = 0.f;
-        }
-        const uint32_t half_bar = bars + 8 * (C::B_P_HALF + ti);
+        st &= ~FIRST;
+        const float neg_m = m == -INFINITY ? 0.f : -m;
         float sum0, sum1;
-        if (full)
-          row_exp_store<false>(s, mul, neg_m, hi, tS, sum0, sum1, half_bar, [] {}, [] {});
+        // Where scores are so large that m is a rounded product, each score is
+        // rounded as m was, or the largest would lie half a step of m off it.
+        if (full && !(st & LARGE))
+          row_exp_store<false>(s, sl2, neg_m, hi, tS, sum0, sum1, bar + 8 * C::B_P_HALF, [] {}, [] {});
         else
-          row_exp_store<true>(s, mul, neg_m, hi, tS, sum0, sum1, half_bar, [] {}, [] {}, lo);
+          row_exp_store<true, true>(s, sl2, neg_m, hi, tS, sum0, sum1, bar + 8 * C::B_P_HALF, [] {}, [] {}, lo);
         l += sum0 + sum1;
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(bars + 8 * (C::B_P + ti));
+        mbar_arrive(bar + 8 * C::B_P);
       }
       if (m == -INFINITY && l != l) m = 0.f;  // a row of NaN scores has no maximum, its sums are NaN
-      if (ok && t0 < t1) {
-        ok = wait(C::B_O + ti, 0);
+      const bool some = sg.t0 < sg.t1;
+      if ((st & OK) && some) {
+        if (!tile_wait(C::B_O, 0)) st &= ~OK;
         tc_fence_after();
       }
-      if (ok) {
-        if (p.pieces > 1) {
-          // chunk-major: 4 columns of one row are 16 bytes, the 256 rows of a chunk are contiguous
-          const long long slot = (static_cast<long long>(want) * a.kv_heads + head) * p.pieces + piece;
-          float* dst = p.part_o + slot * 2 * M_ROWS * D + (ti * M_ROWS + row) * 4;
-          *reinterpret_cast<float2*>(p.part_ml + (slot * 2 * M_ROWS + ti * M_ROWS + row) * 2) = make_float2(m, l);
-          if (t0 < t1) {
+      const Place at(sg, a);
+      const uint32_t tO = tS + 256 - at.tile * (128 - D);
+      if (!(st & OK)) {
+        // a wait ran out: nothing is stored
+      } else if (sg.pieces == 1) {
+        // through this warp's staging tile, so that 8 lanes store 128 contiguous bytes of a row
+        const float inv = m == -INFINITY ? 0.f : (a.v_scale ? a.v_scale[sg.head] : 1.f) / l;
+        uint16_t* const o_head = a.o + sg.first * a.o_stride_t + static_cast<long long>(sg.head) * a.group * a.o_stride_h;
+        const uint32_t stg = s0 + C::STAGE_OFF + warp * 4096;
+#pragma unroll 1
+        for (int hf = 0; hf < D / 64; ++hf) {
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(tO + 32 * c, o);
+          for (int cc = 0; cc < 2; ++cc) {
+            uint32_t o[32];
+            if (some) {
+              tmem_ld32(tO + 64 * hf + 32 * cc, o);
               tmem_wait_ld();
               reg_fence32(o);
+            }
+            // a row that sees no key is zero, whatever the accumulator holds
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                *reinterpret_cast<float4*>(dst + (c * 8 + e) * 2 * M_ROWS * 4) =
-                    make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
-                                __uint_as_float(o[4 * e + 3]));
+            for (int e = 0; e < 32; ++e) o[e] = m == -INFINITY ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t h[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                h[i] = float2_to_pair<BF16>(__uint_as_float(o[8 * e + 2 * i]), __uint_as_float(o[8 * e + 2 * i + 1]));
+              st_shared_v4(stg + lane * 128 + (((cc * 4 + e) ^ (lane & 7)) << 4), h[0], h[1], h[2], h[3]);
             }
           }
-        } else {
-          // through this warp's staging tile, so that 8 lanes store 128 contiguous bytes of a row
-          const float inv = m == -INFINITY ? 0.f : (a.v_scale ? a.v_scale[head] : 1.f) / l;
-          const uint32_t stg = s0 + C::STAGE_OFF + warp * 4096;
+          __syncwarp();
 #pragma unroll
-          for (int hf = 0; hf < D / 64; ++hf) {
-#pragma unroll
-            for (int cc = 0; cc < 2; ++cc) {
-              uint32_t o[32];
-              if (t0 < t1) {
-                tmem_ld32(tO + 64 * hf + 32 * cc, o);
-                tmem_wait_ld();
-                reg_fence32(o);
-              }
-              // a row that sees no key is zero, whatever the accumulator holds
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = m == -INFINITY ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                uint32_t h[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  h[i] = float2_to_pair<BF16>(__uint_as_float(o[8 * e + 2 * i]), __uint_as_float(o[8 * e + 2 * i + 1]));
-                st_shared_v4(stg + lane * 128 + (((cc * 4 + e) ^ (lane & 7)) << 4), h[0], h[1], h[2], h[3]);
-              }
-            }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = i * 4 + (lane >> 3), ch = lane & 7;
-              const uint4 x = ld_shared_v4(stg + r * 128 + ((ch ^ (r & 7)) << 4));
-              const int at = row0 + ti * M_ROWS + quad * 32 + r;
-              if (at < total_rows)
-                *reinterpret_cast<uint4*>(a.o + (rows.first + at / a.group) * a.o_stride_t +
-                                          (static_cast<long long>(head) * a.group + at % a.group) * a.o_stride_h +
-                                          hf * 64 + ch * 8) = x;
-            }
-            __syncwarp();
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3), ch = lane & 7;
+            const uint4 x = ld_shared_v4(stg + r * 128 + ((ch ^ (r & 7)) << 4));
+            const int to = at.my_row - lane + r;
+            if (to < at.total)
+              *reinterpret_cast<uint4*>(o_head + a.token_of(to) * a.o_stride_t +
+                                        (to - a.token_of(to) * a.group) * a.o_stride_h + hf * 64 + ch * 8) = x;
           }
+          __syncwarp();
+        }
+      } else {
+        // a piece: unnormalised O, m and l to the workspace, chunk-major (4 columns
+        // of one row are 16 bytes, the 256 rows of a chunk are contiguous)
+        const long long slot = static_cast<long long>(sg.tail) * MAX_PIECES + sg.piece;
+        *reinterpret_cast<float2*>(p.part_ml + (slot * 2 * M_ROWS + at.tile * M_ROWS + at.row) * 2) = make_float2(m, l);
+        if (some) {
+          float* dst = p.part_o + slot * 2 * M_ROWS * D + (at.tile * M_ROWS + at.row) * 4;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + 32 * c, o);
+            tmem_wait_ld();
+            reg_fence32(o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<float4*>(dst + (c * 8 + e) * 2 * M_ROWS * 4) =
+                  make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
+                              __uint_as_float(o[4 * e + 3]));
+          }
+        }
+        // The rendezvous orders the warpgroup's stores before one thread's
+        // fence, and that before its count.
+        mbar_arrive(bar + 8 * C::B_WG);
+        bool met = tile_wait(C::B_WG, 0);
+        if (met && at.row == 0) {
+          unsigned long long* count = p.done + sg.tail * 2 + at.tile;
+          __threadfence();
+          const bool last = static_cast<int>(atomicAdd(count, 1ull) & 0xffffull) + 1 == sg.pieces;
+          if (last) {
+            __threadfence();
+            atomicExch(count, p.epoch << 16);
+          }
+          last_flag[at.tile] = last;
+        }
+        mbar_arrive(bar + 8 * C::B_WG);
+        met = met && tile_wait(C::B_WG, 1);
+        if (met && last_flag[at.tile] && at.live) {
+          const int t = a.token_of(at.my_row);
+          join_row<D, BF16>(p, sg.tail, sg.pieces, at.tile * M_ROWS + at.row, sg.head,
+                            a.o + (sg.first + t) * a.o_stride_t +
+                                (static_cast<long long>(sg.head + 1) * a.group + at.my_row - (t + 1) * a.group) * a.o_stride_h);
         }
       }
     }
@@ -624,63 +802,17 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
   }
 }
 
-// Joins the pieces of a unit: blockIdx.x is (block, kv head), blockIdx.y 16
-// columns; one thread per row. Pieces are added in their order.
-template <int D, bool BF16>
-__global__ void __launch_bounds__(2 * M_ROWS) cache4_many_join_kernel(const ManyParams p) {
-  const AttnParams& a = p.a;
-  griddep_wait();
-  if (threadIdx.x == 0) griddep_launch_dependents();
-  const int head = static_cast<int>(blockIdx.x) % a.kv_heads, want = static_cast<int>(blockIdx.x) / a.kv_heads;
-  Unit u;
-  if (!find_unit<2 * M_ROWS>(p, want, &u)) return;
-  const Rows rows = rows_of(a, u.r);
-  const int row = threadIdx.x, at = u.block * 2 * M_ROWS + row;
-  if (at >= rows.n * a.group) return;
-  const long long slot0 = (static_cast<long long>(want) * a.kv_heads + head) * p.pieces;
-  float m = -INFINITY, l = 0.f, x[16];
-#pragma unroll
-  for (int e = 0; e < 16; ++e) x[e] = 0.f;
-  for (int k = 0; k < p.pieces; ++k) m = fmaxf(m, p.part_ml[((slot0 + k) * 2 * M_ROWS + row) * 2]);
-  for (int k = 0; k < p.pieces; ++k) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((slot0 + k) * 2 * M_ROWS + row) * 2);
-    if (ml.x == -INFINITY) continue;  // the piece saw no key of this row
-    const float f = ex2_approx(ml.x - m);
-    l += ml.y * f;
-    const float* src = p.part_o + (slot0 + k) * 2 * M_ROWS * D + row * 4;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float4 y = *reinterpret_cast<const float4*>(src + (blockIdx.y * 4 + q) * 2 * M_ROWS * 4);
-      x[4 * q] += y.x * f;
-      x[4 * q + 1] += y.y * f;
-      x[4 * q + 2] += y.z * f;
-      x[4 * q + 3] += y.w * f;
-    }
-  }
-  const float inv = m == -INFINITY ? 0.f : (a.v_scale ? a.v_scale[head] : 1.f) / l;
-  uint32_t h[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) h[e] = float2_to_pair<BF16>(x[2 * e] * inv, x[2 * e + 1] * inv);
-  uint4* dst = reinterpret_cast<uint4*>(a.o + (rows.first + at / a.group) * a.o_stride_t +
-                                        (static_cast<long long>(head) * a.group + at % a.group) * a.o_stride_h +
-                                        blockIdx.y * 16);
-  dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
-  dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
-}
-
 // -------------------------------------------------------------------- host
 ManyPlan many_plan(int tokens, int requests, int group, int kv_heads, int D, int sms) {
   ManyPlan pl{};
   const long long blocks = static_cast<long long>(tokens) * group / (2 * M_ROWS) + requests;
-  if (blocks * kv_heads > INT_MAX / 8) return pl;
-  pl.max_blocks = static_cast<int>(blocks);
-  const long long units = blocks * kv_heads;
-  pl.pieces = units * 2 <= sms ? static_cast<int>(sms / units < 8 ? sms / units : 8) : 1;
-  if (pl.pieces > 1) {
-    const size_t rows = static_cast<size_t>(units) * pl.pieces * 2 * M_ROWS;
-    pl.ml_off = rows * D * sizeof(float);
-    pl.bytes = pl.ml_off + rows * 2 * sizeof(float);
-  }
+  if (blocks * kv_heads > INT_MAX / 1024 - sms * MAX_PIECES) return pl;
+  pl.max_units = static_cast<int>(blocks * kv_heads);
+  // cut units: fewer than SMs
+  const size_t rows = static_cast<size_t>(pl.max_units < sms ? pl.max_units : sms) * MAX_PIECES * 2 * M_ROWS;
+  pl.ml_off = rows * D * sizeof(float);
+  pl.done_off = pl.ml_off + rows * 2 * sizeof(float);
+  pl.bytes = pl.done_off + static_cast<size_t>(sms) * 2 * sizeof(unsigned long long);
   return pl;
 }
 
@@ -688,10 +820,10 @@ template <int D, bool BF16>
 static int launch_many_t(const ManyParams& p, cudaStream_t stream) {
   static SmemAttribute smem;
   if (!smem.set(cache4_many_kernel<D, BF16>, Many<D>::SMEM)) return GFX906_B200_ECUDA;
-  const int units = p.max_blocks * p.a.kv_heads;
-  const int rc = launch(cache4_many_kernel<D, BF16>, dim3(units * p.pieces), dim3(M_THREADS), Many<D>::SMEM, stream, p);
-  if (rc != GFX906_B200_OK || p.pieces == 1) return rc;
-  return launch(cache4_many_join_kernel<D, BF16>, dim3(units, D / 16), dim3(2 * M_ROWS), 0, stream, p);
+  // the units, and the pieces of those of the last wave
+  const long long cut = static_cast<long long>(p.max_units < p.sms ? p.max_units : p.sms - 1) * (MAX_PIECES - 1);
+  const long long ctas = p.max_units + (cut < CUT_CTAS * p.sms ? cut : CUT_CTAS * p.sms);
+  return launch(cache4_many_kernel<D, BF16>, dim3(static_cast<unsigned>(ctas)), dim3(M_THREADS), Many<D>::SMEM, stream, p);
 }
 
 int launch_many(const ManyParams& p, int D, int dtype, cudaStream_t stream) {

@@ -9,16 +9,20 @@ namespace c4 {
 
 struct ManyParams {
   AttnParams a;
-  int min_rows;     // requests with at most this many query rows are another kernel's
-  int max_blocks;   // blocks of 256 query rows of all requests, at most
-  int pieces;       // runs that each unit's keys are cut into
-  float* part_o;    // [blocks * kv_heads * pieces][D / 4][256][4], pieces > 1
-  float* part_ml;   // [blocks * kv_heads * pieces][256][2]
+  int min_rows;      // requests with at most this many query rows are another kernel's
+  int max_units;     // units of 256 query rows and a kv head, at most
+  int sms;
+  float* part_o;     // [sms][MAX_PIECES][D / 4][256][4]
+  float* part_ml;    // [sms][MAX_PIECES][256][2]
+  // [sms][2] pieces of a cut unit that are in the workspace, for each of its query
+  // tiles, tagged with the launch as in the other kernel
+  unsigned long long* done;
+  unsigned long long epoch;
   unsigned long long timeout_ns;
 };
 struct ManyPlan {
-  int max_blocks, pieces;  // max_blocks 0: too large a call
-  size_t ml_off, bytes;    // workspace
+  int max_units;  // 0: too large a call
+  size_t ml_off, done_off, bytes;  // workspace
 };
 ManyPlan many_plan(int tokens, int requests, int group, int kv_heads, int D, int sms);
 int launch_many(const ManyParams& p, int D, int dtype, cudaStream_t stream);
