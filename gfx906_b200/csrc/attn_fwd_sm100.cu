@@ -2101,7 +2101,8 @@ const char* gfx906_b200_attn_error_string(int status) {
   }
 }
 
-int gfx906_b200_internal_cache4_status(int reset);  // cache4_many.cu
+int gfx906_b200_internal_cache4_status(int reset);      // cache4_many.cu
+int gfx906_b200_internal_cache4_few_status(int reset);  // cache4_attn.cu
 
 int gfx906_b200_attn_device_status(int reset) {
   if (cudaDeviceSynchronize() != cudaSuccess) return GFX906_B200_ECUDA;
@@ -2114,9 +2115,9 @@ int gfx906_b200_attn_device_status(int reset) {
         cudaMemcpyToSymbol(fa::g_timeout_info, zeros, sizeof(zeros)) != cudaSuccess)
       return GFX906_B200_ECUDA;
   }
-  const int cache4 = gfx906_b200_internal_cache4_status(reset);
-  if (cache4 < 0) return GFX906_B200_ECUDA;
-  return (st || cache4) ? GFX906_B200_ETIMEOUT : GFX906_B200_OK;
+  const int many = gfx906_b200_internal_cache4_status(reset), few = gfx906_b200_internal_cache4_few_status(reset);
+  if (many < 0 || few < 0) return GFX906_B200_ECUDA;
+  return (st || many || few) ? GFX906_B200_ETIMEOUT : GFX906_B200_OK;
 }
 
 int gfx906_b200_attn_timeout_info(int* out6) {

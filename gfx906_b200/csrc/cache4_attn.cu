@@ -55,6 +55,7 @@ struct FewParams {
   // whoever joins a unit sets its word to none again, for a replay of the launch.
   unsigned long long* done;
   unsigned long long epoch;
+  unsigned long long timeout_ns;
 };
 
 template <int D, int NT>
@@ -78,13 +79,29 @@ struct Few {
   static_assert(PER_SM >= 1 && ROWS * LD * 4 <= RING, "a warp's merge buffer is its ring");
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ unsigned int g_cache4_few_status = 0;  // 1: a wait for a copy ran out
+
+// Contiguous copy global -> shared (16-byte aligned, bytes a multiple of 16),
+// counted on `bar`.
+__device__ __forceinline__ void copy_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Whole warp: waits at most `limit_ns` for the phase of that parity.
+__device__ __forceinline__ bool wait_copy(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
+  bool ok = fa::mbar_try_wait(bar, parity);
+  if (!ok) {
+    const uint64_t t0 = fa::globaltimer_ns();
+    uint32_t n = 0;
+    while (!(ok = fa::mbar_try_wait(bar, parity))) {
+      if ((++n & 31u) == 0u && (fa::globaltimer_ns() - t0 > limit_ns || n > (1u << 24))) {
+        atomicOr(&g_cache4_few_status, 1u);
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
 }
 // W words at a, W = 2 or 4.
 template <int W>
@@ -423,6 +440,7 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
   __shared__ Share found;
   __shared__ int found_base, found_r;
   __shared__ bool joins;
+  __shared__ __align__(8) unsigned long long copied_bars[WARPS][C::STAGES];
   const AttnParams& a = p.a;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int n = lane >> 2, c = lane & 3;
@@ -431,6 +449,16 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
   const uint8_t* ring_at = smem + warp * C::RING;
   float2* ml = reinterpret_cast<float2*>(smem + C::ML_OFF);
   float* rowf = reinterpret_cast<float*>(smem + C::ROWF_OFF);
+  // this warp's stages: a barrier for each, and the parity of its next phase
+  const uint32_t copied = fa::smem_u32(copied_bars[warp]);
+  uint32_t phases = 0;
+  bool late = false;
+  if (lane == 0) {
+    for (int i = 0; i < C::STAGES; ++i) fa::mbar_init(copied + 8 * i, 1);
+    fa::fence_barrier_init();
+    fa::fence_proxy_async_smem();
+  }
+  __syncwarp();
   fa::griddep_wait();
   if (threadIdx.x == 0) fa::griddep_launch_dependents();
 
@@ -549,7 +577,7 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
     uint32_t good = 0;  // bit: the step in that stage has a page
     int issued = 0;
     auto issue = [&]() {
-      if (issued < my_steps) {
+      if (issued < my_steps && !late) {
         if (issued >= ids_at + 32) {
           ids_at = issued;
           const int k = k_begin + warp + WARPS * (ids_at + lane);
@@ -564,13 +592,13 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
           const uint8_t* src = a.cache + (static_cast<long long>(page) * a.kv_heads + head) * L::PAGE_BYTES +
                                (k & 1) * C::STEP_BYTES;
           const uint32_t dst = ring + stage * C::STEP_BYTES;
-#pragma unroll
-          for (int i = 0; i < (C::STEP_BYTES + 511) / 512; ++i)
-            if (i * 512 + lane * 16 < C::STEP_BYTES) cp_async16(dst + i * 512 + lane * 16, src + i * 512 + lane * 16);
+          if (lane == 0) {
+            fa::mbar_arrive_expect_tx(copied + 8 * stage, C::STEP_BYTES);
+            copy_bulk(dst, src, C::STEP_BYTES, copied + 8 * stage);
+          }
         }
         ++issued;
       }
-      cp_async_commit();
     };
 #pragma unroll
     for (int i = 0; i < C::STAGES - 1; ++i) issue();
@@ -640,12 +668,16 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
         for (int e = 0; e < 4; ++e) acc.o[t][nt][e] = 0.f;
 
     // ---- this warp's steps
-    for (int i = 0; i < my_steps; ++i) {
+    for (int i = 0; i < my_steps && !late; ++i) {
       issue();
-      cp_async_wait<C::STAGES - 1>();
       __syncwarp();
       const int stage = i % C::STAGES;
       if ((good >> stage) & 1u) {
+        if (!wait_copy(copied + 8 * stage, (phases >> stage) & 1u, p.timeout_ns)) {
+          late = true;
+          break;
+        }
+        phases ^= 1u << stage;
         const int key0 = (k_begin + warp + WARPS * i) * STEP;
         if (key0 + STEP > least)
           step<D, NT, true>(acc, ring_at + stage * C::STEP_BYTES, smem + C::Q_OFF, lane, factor, key0, len, limit);
@@ -654,7 +686,12 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
       }
       __syncwarp();  // the stage is free for the next copy
     }
-    cp_async_wait<0>();
+    // a copy that did not come in time: the status word is set, this warp takes no
+    // further steps, and waits (for as long again) until none is in flight
+    if (late) {
+      for (int stage = 0; stage < C::STAGES; ++stage)
+        if ((good >> stage) & 1u) wait_copy(copied + 8 * stage, (phases >> stage) & 1u, p.timeout_ns);
+    }
 
     // ---- the four warps' sums become one
 #pragma unroll
@@ -736,7 +773,8 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
                           split.owner(pos - off + sh.steps - 1) - first_block + 1, sh.first, row0, nrows, head, vf);
     }
     pos += stop - off;
-    __syncthreads();  // the merge buffers, Q and row factors are free
+    fa::fence_proxy_async_smem();  // what was stored in the rings comes before the next copies
+    __syncthreads();               // the merge buffers, Q and row factors are free
   }
   if (a.zero_rest) {
     const int from = min(max(a.query_start[a.requests], 0), a.tokens);
@@ -839,6 +877,7 @@ static int attn(const gfx906_b200_cache4_attn_args& g, void* ws, size_t ws_bytes
   p.part_ml = reinterpret_cast<float*>(base + pl.ml_off);
   p.done = reinterpret_cast<unsigned long long*>(base + pl.done_off);
   p.epoch = gfx906_b200_internal_next_epoch() & 0xffffffffffffull;
+  p.timeout_ns = gfx906_b200_internal_timeout_ns();
   if (g.D == 128)
     return pl.nt == 1 ? launch_few_t<128, 1>(p, g.dtype, pl.blocks, stream)
                       : launch_few_t<128, 2>(p, g.dtype, pl.blocks, stream);
@@ -849,6 +888,15 @@ static int attn(const gfx906_b200_cache4_attn_args& g, void* ws, size_t ws_bytes
 }  // namespace c4
 
 extern "C" {
+
+// 1 when a wait of these kernels ran out; < 0 on a CUDA error.
+int gfx906_b200_internal_cache4_few_status(int reset) {
+  unsigned int st = 0;
+  const unsigned int zero = 0;
+  if (cudaMemcpyFromSymbol(&st, c4::g_cache4_few_status, sizeof(st)) != cudaSuccess) return -1;
+  if (reset && cudaMemcpyToSymbol(c4::g_cache4_few_status, &zero, sizeof(zero)) != cudaSuccess) return -1;
+  return st ? 1 : 0;
+}
 
 size_t gfx906_b200_cache4_attn_workspace_size(const gfx906_b200_cache4_attn_args* args) {
   int sms = 0;
