@@ -25,7 +25,7 @@ waiting for the GPU::
 
 A number is an e2m1 code times an e4m3 scale, shared by 16 neighbouring
 channels of a token, times a float32 factor per kv head (``k_scale``,
-``v_scale``; 1 where they are None). The factor serves numbers whose scale
+``v_scale``, positive; 1 where they are None). The factor serves numbers whose scale
 leaves e4m3's range: the largest magnitude of a head divided by 2688 keeps all
 of it. The byte layout of a page is in ``csrc/cache4.cuh``.
 

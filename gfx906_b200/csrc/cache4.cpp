@@ -2,6 +2,7 @@
 // (include/gfx906_b200_cache4.h). Like `attn`: inputs are checked, launched on
 // the current stream of their device, and failures raise RuntimeError.
 #include <torch/extension.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
@@ -187,8 +188,8 @@ Tensor attn_cache4(Tensor q, Tensor cache, Tensor tables, Tensor lengths, Tensor
   const float* vs = check_scale(v_scale, cache, kv_heads, "v_scale");
   if (out.has_value())
     TORCH_CHECK(out->is_cuda() && out->device() == q.device() && out->dtype() == q.dtype() && out->sizes() == q.sizes() &&
-                    rows_ok(*out),
-                "cache4: out must be a tensor like q with rows that start on 16 bytes");
+                    rows_ok(*out) && at::has_internal_overlap(*out) != at::MemOverlap::Yes,
+                "cache4: out must be a tensor like q with rows of its own that start on 16 bytes");
   const c10::cuda::CUDAGuard guard(cache.device());
   const Tensor qc = with_rows(q);
   Tensor o = out.has_value() ? *out : new_tensor(q.sizes(), q.scalar_type(), q);

@@ -19,6 +19,13 @@
 // eight rows (all heads of a group for one token) leave no half of the
 // instruction empty. Codes become fp16 by one conversion and one exact product
 // per pair, in registers.
+//
+// Measured (B200, D = 128, 8 kv heads of 4 query heads): 32 requests of up to
+// 16384 tokens 79 us, 4.7 TB/s of cache; 131072 tokens of one request 40 us, 3.7
+// TB/s. With the arithmetic taken out the same copies take 69 and 35 us, with the
+// copies taken out the arithmetic takes 74 and 40 (about 580 instructions of a
+// warp per step, 270 of them on the ALU pipe, 128 of these conversions): it is
+// bound by both, and by the 8 us before the first step and behind the last.
 #include <limits.h>
 #include <math.h>
 
@@ -31,15 +38,13 @@
 namespace c4 {
 
 // Requests with more query rows (tokens times heads of a group) go to the
-// tensor-memory kernel of cache4_many.cu.
+// tensor-memory kernel of cache4_many.cu, which takes 256 rows at the price of
+// one. Measured at D = 128, us here and there for 48, 64, 96, 128 rows a request:
+// 1 x 8192 keys, 8 kv heads: 30, 33, 36, 41 and 41, 41, 41, 43; 8 x 4096, 8: 53,
+// 64, 85, 106 and 52, 52, 52, 53; 32 x 2048, 8: 94, 119, 167, 213 and 124, 125,
+// 126, 130; 4 x 32768, 2: 52, 60, 80, 100 and 79, 78, 79, 80.
 constexpr int FEW_ROWS = 64;
 
-#ifndef FEW_WARPS
-#define FEW_WARPS 4
-#endif
-#ifndef FEW_MIN
-#define FEW_MIN 1
-#endif
 constexpr int MAX_REQUESTS = 8192;
 constexpr int STEP = 32;                // tokens of a step
 constexpr float REACH = 8.f;            // see step()
@@ -61,11 +66,16 @@ struct FewParams {
 template <int D, int NT>
 struct Few {
   using L = Layout<D>;
-  static constexpr int WARPS = NT == 1 || FEW_WARPS == 4 ? FEW_WARPS : FEW_WARPS == 8 ? 6 : 12;
+  // Four warps to a block. Eight, in half as many blocks, join fewer pieces of
+  // one long context (131072 keys: 38 us, not 40) but wait longer at each unit's
+  // end (ragged batch of 32: 82 us, not 79; drafts for 16 requests: 49, not 43).
+  static constexpr int WARPS = 4;
   static constexpr int THREADS = WARPS * 32;
-  static constexpr int PER_SM = (NT == 1 ? 16 : 12) / WARPS;  // blocks that share an SM
+  static constexpr int PER_SM = NT == 1 ? 4 : 3;  // blocks that share an SM, by registers
   static constexpr int MAX_CHUNKS = (MAX_REQUESTS + THREADS - 1) / THREADS;
-  static constexpr int MIN_STEPS = WARPS * FEW_MIN;  // steps of a unit that are worth a block of their own
+  // Steps of a unit that are worth a block of their own: one for each warp (two:
+  // 8 heads x 1000 keys 10.2 us, not 9.7).
+  static constexpr int MIN_STEPS = WARPS;
   static constexpr int ROWS = 8 * NT;
   static constexpr int STEP_BYTES = 2 * L::BLOCK_BYTES;
   static constexpr int STAGES = NT == 1 ? 2 : 3;  // four or three blocks share an SM
@@ -848,7 +858,9 @@ static int attn(const gfx906_b200_cache4_attn_args& g, void* ws, size_t ws_bytes
   const int rc = gfx906_b200_internal_device(&sms);
   if (rc != GFX906_B200_OK) return rc;
   const Plan pl = plan_of(g, sms);
-  if (!pl.fits || (static_cast<long long>(g.max_tokens) * (g.heads / g.kv_heads) > FEW_ROWS && !pl.many.max_units) || !ws || ws_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(ws) & 255u)) return GFX906_B200_EINVAL;
+  const bool any_many = static_cast<long long>(g.max_tokens) * (g.heads / g.kv_heads) > FEW_ROWS;
+  if (!pl.fits || (any_many && !pl.many.max_units)) return GFX906_B200_EINVAL;
+  if (!ws || ws_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(ws) & 255u)) return GFX906_B200_EINVAL;
   FewParams p{};
   p.a = {static_cast<const uint16_t*>(g.q), static_cast<uint16_t*>(g.o), static_cast<const uint8_t*>(g.cache), g.tables,
          g.lengths, g.query_start, g.k_scale, g.v_scale, g.q_stride_t, g.q_stride_h, g.o_stride_t, g.o_stride_h,

@@ -155,6 +155,28 @@ def test_write_every_byte(D, dtype, T, H):
             assert torch.equal(got.cpu(), torch.from_numpy(exact).float().to(out))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_write_rounds_every_quotient_as_a_division(dtype):
+    """Every finite 16-bit number beside each of several largest ones, under factors of any size:
+    the codes are those of the 32-bit quotient."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    numbers = bits[torch.isfinite(bits)]
+    numbers = numbers[numbers.abs() <= 3.0]  # the 16th of a group is its largest
+    numbers = numbers[:numbers.numel() // 15 * 15].view(-1, 15)
+    for factor in (1.0, 0.3, 7.1e-3, 1.7e5, 3e-30, 2e30):
+        for most in (3.0, 3.7, 5.99):
+            x = torch.cat([numbers, torch.full((len(numbers), 1), most, dtype=dtype)], 1)
+            x = x[:x.shape[0] // 4 * 4].reshape(-1, 1, 64)
+            T = x.shape[0]
+            cache = g.cache4_alloc(-(-T // 64), 1, 64)
+            f = torch.tensor([factor], device="cuda")
+            g.cache4_write(x.cuda(), -x.cuda(), cache, ints(range(T)), f, f)
+            k, v = g.cache4_read(cache, ints(range(T)), f, f, dtype=torch.float32)
+            codes, scales = oracle.quantise(x, f.cpu().numpy())
+            want = torch.from_numpy(oracle.numbers(codes, scales, f.cpu().numpy())).float()
+            assert torch.equal(k.cpu(), want) and torch.equal(v.cpu(), -want), (factor, most)
+
+
 def test_write_without_factors_and_from_strided_rows():
     T, H, D = 40, 4, 128
     qkv = torch.randn(T, 3 * H * D + 64, generator=torch.Generator().manual_seed(5)).half()
@@ -479,6 +501,20 @@ def test_attention_survives_wild_index_tensors():
     torch.cuda.synchronize()
 
 
+def test_attention_in_place():
+    for counts in ([1, 2], [100, 2]):
+        p = Problem(counts, [3000, 90], 2, 2, 64, torch.float16)
+        want = p.run(max_tokens=max(counts))
+        q = p.q.cuda()
+        p.run(q=q, max_tokens=max(counts), out=q)
+        assert torch.equal(q, want)
+
+
+def test_attention_of_many_heads_on_one():
+    p = Problem([1, 2], [700, 90], 1, 96, 64, torch.bfloat16)  # more rows of one token than the small kernel takes
+    p.check(p.run(max_tokens=2))
+
+
 def test_attention_is_deterministic_and_ignores_the_hint():
     p = Problem([1, 1, 2], [3000, 77, 1500], 2, 3, 128, torch.float16)
     a, b = p.run(max_tokens=2), p.run(max_tokens=2)
@@ -498,16 +534,18 @@ def test_attention_refusals():
                 {"query_start": ints([0, 1])}, {"query_start": ok["query_start"].cpu()}, {"scale": float("nan")},
                 {"scale": 1e300}, {"max_tokens": -1}, {"out": q.float()}, {"out": q[:2]}, {"out": q.cpu()},
                 {"out": torch.empty(3, 4, 128, dtype=torch.float16, device="cuda")[..., ::2]},
+                {"out": torch.empty(1, 4, 64, dtype=torch.float16, device="cuda").expand(3, 4, 64)},
                 {"k_scale": torch.ones(4, device="cuda")}, {"v_scale": torch.ones(2)},
                 {"cache": p.cache.transpose(0, 1)}, {"cache": p.cache[..., :100].contiguous()}):
         with pytest.raises(RuntimeError):
             g.attn_cache4(**{**ok, **bad})
 
 
-def test_attention_on_other_streams_and_in_graphs():
-    p = Problem([1, 1], [5000, 300], 2, 4, 128, torch.float16)
+@pytest.mark.parametrize("counts", [[1, 1], [70, 1], [3, 300]])  # one kernel, both, both
+def test_attention_on_other_streams_and_in_graphs(counts):
+    p = Problem(counts, [5000, 300], 2, 4, 128, torch.float16)
     q2 = torch.randn(p.q.shape, generator=torch.Generator().manual_seed(9)).half()
-    want, want2 = p.run(max_tokens=1), p.run(q=q2, max_tokens=1)
+    want, want2 = p.run(max_tokens=max(counts)), p.run(q=q2, max_tokens=max(counts))
     kf, vf = p.factors()
     fixed = (p.cache, ints(p.tables), ints(p.lengths), ints(p.query_start), p.scale)
     side = [torch.cuda.Stream() for _ in range(2)]
@@ -518,14 +556,14 @@ def test_attention_on_other_streams_and_in_graphs():
     for _ in range(5):  # two calls at once, each on its own stream
         for i in range(2):
             with torch.cuda.stream(side[i]):
-                outs[i].append(g.attn_cache4(qs[i], *fixed, k_scale=kf, v_scale=vf, max_tokens=1))
+                outs[i].append(g.attn_cache4(qs[i], *fixed, k_scale=kf, v_scale=vf, max_tokens=max(counts)))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs[0]) and all(torch.equal(o, want2) for o in outs[1])
     graphs, results = [], []
     for i in range(2):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            results.append(g.attn_cache4(qs[i], *fixed, k_scale=kf, v_scale=vf, max_tokens=1))
+            results.append(g.attn_cache4(qs[i], *fixed, k_scale=kf, v_scale=vf, max_tokens=max(counts)))
         graphs.append(graph)
     for _ in range(3):
         results[0].zero_()
