@@ -127,8 +127,9 @@ def attn_cache4(q, cache, tables, lengths, query_start, scale, causal=True, k_sc
     tokens in the cache.
 
     q [tokens, heads, head_dim] is fp16 or bf16 with any strides; rows
-    query_start[r] to query_start[r + 1] belong to request r, which attends to
-    its first lengths[r] tokens in the pages tables[r]. heads is a multiple of
+    query_start[r] to query_start[r + 1] (which does not decrease; it starts at
+    0) belong to request r, which attends to its first lengths[r] tokens in the
+    pages tables[r]. heads is a multiple of
     the cache's kv heads; consecutive query heads share one. With ``causal`` a
     request's last row sees all its tokens and each row before it one token
     less; without, every row sees them all. Rows that see none are zero.

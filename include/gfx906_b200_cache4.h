@@ -65,7 +65,8 @@ GFX906_B200_API int gfx906_b200_cache4_read(const void* cache, int pages, const 
                                             int dtype, cudaStream_t stream);
 
 /* Attention of new tokens against the cache. Request r's query rows are
- * query_start[r] .. query_start[r + 1] of q [tokens, heads, D]; it attends to
+ * query_start[r] .. query_start[r + 1] of q [tokens, heads, D] (query_start does
+ * not decrease; whatever it holds, no row outside q is touched); it attends to
  * its lengths[r] tokens in tables[r * width ...]. Query head h uses kv head
  * h / (heads / kv_heads). With causal != 0 the last query row sees every
  * token and each row before it one less; rows that see none get zeros. */

@@ -498,6 +498,14 @@ def test_attention_survives_wild_index_tensors():
     for lengths, starts in (([2 ** 31 - 1, -5], [0, 1, 3]), ([100, 90], [-3, 2 ** 31 - 1, 3]), ([100, 90], [3, 2, 1])):
         out = g.attn_cache4(p.q.cuda(), p.cache, ints(p.tables), ints(lengths), ints(starts), p.scale, k_scale=kf, v_scale=vf)
         assert out.shape == p.q.shape and width
+    p = Problem([100, 200], [100, 290], 1, 2, 128, torch.float16)
+    for lengths, starts in (([2 ** 31 - 1, -5], [0, 100, 300]), ([100, 90], [-3, 2 ** 31 - 1, 3]),
+                            ([100, 90], [300, 200, 100]), ([100, 290], [0, 300, 300]), ([100, 290], [250, 300, 2 ** 31 - 1])):
+        out = g.attn_cache4(p.q.cuda(), p.cache, ints(p.tables), ints(lengths), ints(starts), p.scale)
+        assert out.shape == p.q.shape
+    # decreasing starts may make the requests' rows more than there are
+    starts = [0, 300] * 50 + [0]
+    out = g.attn_cache4(p.q.cuda(), p.cache, ints(p.tables[:1] * 100), ints([100] * 100), ints(starts), p.scale)
     torch.cuda.synchronize()
 
 
