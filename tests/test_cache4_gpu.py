@@ -332,6 +332,14 @@ def test_attention_many_tokens(shape, D, dtype):
     assert torch.equal(p.run(), p.run())
 
 
+def test_attention_many_tokens_of_many_requests():
+    """More requests than are sorted by length, short and long ones mixed."""
+    rng = random.Random(7)
+    counts = [rng.choice([1, 2, 65, 70]) for _ in range(150)]
+    p = Problem(counts, [n + rng.randint(0, 100) for n in counts], 1, 1, 64, torch.float16)
+    p.check(p.run(), rows=[0, 1, 64, 69])
+
+
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 1.5])
 def test_attention_many_tokens_scales(scale):
     p = Problem([150], [400], 1, 1, 64, torch.float16)
