@@ -47,7 +47,10 @@ constexpr int FEW_ROWS = 64;
 
 constexpr int MAX_REQUESTS = 8192;
 constexpr int STEP = 32;                // tokens of a step
-constexpr float REACH = 8.f;            // see step()
+// Log2 units, see step(): P of a row's largest score is 2^HEAD when the row's
+// reference is set, and stays below 2^REACH, which fp16 holds.
+constexpr float HEAD = 7.f;
+constexpr float REACH = 15.f;
 
 struct FewParams {
   AttnParams a;
@@ -162,7 +165,11 @@ struct Acc {
 // A row's m is a reference that its scores may exceed by REACH (log2 units), not
 // their maximum: P then stays below 2^REACH, O and l carry the same factor, and
 // the maximum across the warp, with the products that follow from it, is taken
-// only in the few steps where a vote finds a score beyond reach.
+// only in the few steps where a vote finds a score beyond reach. The reference is
+// set HEAD below the maximum, so that P uses all of fp16's range: weights down to
+// 2^-21 of the largest are rounded to 2^-11 of themselves, smaller ones by 2^-32
+// of the largest at most (without HEAD 2^-25: a long context's small weights
+// beside one large one would count in l and be lost in O).
 template <int D, int NT, bool MASK>
 __device__ __forceinline__ void step(Acc<D, NT>& acc, const uint8_t* blk, const uint8_t* sq, int lane,
                                      const float (&factor)[NT][2], int key0, int len, const int (&limit)[NT][2]) {
@@ -248,6 +255,7 @@ __device__ __forceinline__ void step(Acc<D, NT>& acc, const uint8_t* blk, const 
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        mx = __fsub_rn(mx, HEAD);
         if (mx > acc.m[nt][i]) {
           const float alpha = fa::ex2_approx(acc.m[nt][i] - mx);
           acc.m[nt][i] = mx;
@@ -258,7 +266,7 @@ __device__ __forceinline__ void step(Acc<D, NT>& acc, const uint8_t* blk, const 
             acc.o[t][nt][2 + i] *= alpha;
           }
         }
-        // rounded as m was, so that the largest score comes to exactly 0, however large
+        // rounded as m was, so that the largest score comes within reach, however large
         const float m_use = acc.m[nt][i] == -INFINITY ? 0.f : acc.m[nt][i];
 #pragma unroll
         for (int b = 0; b < 2; ++b)

@@ -59,7 +59,13 @@ constexpr uint32_t M_REGS_SOFTMAX = 184;
 constexpr uint32_t M_REGS_CONVERT = 64;
 constexpr uint32_t M_REGS_ISSUE = 80;
 constexpr float M_RESCALE = 8.0f;    // log2 units, see the dense kernels
-constexpr float M_LARGE = 67108864.f;  // 2^26: half a 32-bit step is 2 log2 units
+// A row's reference m is set this far below its largest score, so that P, which
+// stays below 2^(M_HEAD + M_RESCALE), uses all of fp16's range: weights down to
+// 2^-21 of the largest are rounded to 2^-11 of themselves, smaller ones by 2^-32
+// of the largest at most (without it by 2^-25: small weights beside a large one
+// would count in l and be lost in O).
+constexpr float M_HEAD = 7.0f;
+constexpr float M_LARGE = 4194304.f;  // 2^22: half a 32-bit step is 1/4 log2 unit, which fits above 2^15
 
 __device__ unsigned int g_cache4_status = 0;  // 1: a wait ran out
 
@@ -712,7 +718,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
         }
         const bool full = __all_sync(0xffffffffu, lo == 0 && hi == BN);
         const float mx = row_extreme(s, hi, full, sl2 >= 0.f, lo);
-        const float m_new = lo < hi ? fmaxf(m, mx * sl2) : m;
+        const float m_new = lo < hi ? fmaxf(m, __fsub_rn(__fmul_rn(mx, sl2), M_HEAD)) : m;
         const bool need = m_new > m + M_RESCALE;
         if (__any_sync(0xffffffffu, need)) {
           float f = 1.f;

@@ -1,0 +1,64 @@
+"""The paged 4-bit cache at the edges of its numbers, sizes and memory (needs a B200)."""
+
+import pytest
+import torch
+
+import gfx906_b200 as g
+from oracle import cache4 as oracle
+
+pytestmark = pytest.mark.gpu
+
+HALF_STEP = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def operator():
+    assert g.load_attention() is not None, g.last_error()
+    yield
+    assert g.device_status(reset=True) == 0
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def held(k, v, pages=None):
+    """k and v [n, heads, D] in a cache of their own, in order: (cache, table, what it holds of k and v in 32 bits)."""
+    n, heads, D = k.shape
+    need = -(-n // 64)
+    cache = g.cache4_alloc(pages or need, heads, D)
+    slots = ints(range(n))
+    g.cache4_write(k.cuda(), v.cuda(), cache, slots)
+    k, v = g.cache4_read(cache, slots, dtype=torch.float32)
+    return cache, ints([list(range(need))]), k.cpu(), v.cpu()
+
+
+# rows of one request: the small kernel in both its instances, the large one (two tiles of rows)
+@pytest.mark.parametrize("rows", [1, 12, 200])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("nats", [9.0, 14.0, 18.0])
+def test_small_weights_beside_large_ones(nats, dtype, D, rows):
+    """One key in 32 outweighs the others by far and has values of zero: all of the output comes from small weights."""
+    n, gen = 1600, torch.Generator().manual_seed(1)
+    k = torch.zeros(n, 1, D)
+    k[5::32, 0, 0] = 6.0
+    v = 1.0 + 0.25 * torch.randn(n, 1, D, generator=gen)
+    v[5::32] = 0
+    cache, table, k, v = held(k.half(), v.half())
+    q = torch.zeros(rows, 1, D)
+    q[:, 0, 0] = 2.0
+    scale = nats / 12
+    # a factor that brings the output to fp16's normal range
+    out = g.attn_cache4(q.to(dtype).cuda(), cache, table, ints([n]), ints([0, rows]), scale, causal=False,
+                        v_scale=torch.tensor([2.0 ** 14], device="cuda"), max_tokens=rows).cpu()
+    v = v[:, 0] * 2.0 ** 14
+    ref, size = oracle.attention(q[:1, 0], k[:, 0], v, scale, False)
+    # Of each weight p (the largest 1): 2^-11 of itself for its rounding to fp16, and 2^-12 for 32-bit scores and
+    # exponentials; where it is below 2^-21, 2^-32. Then one rounding of the output.
+    total = float(torch.softmax(scale * (k[:, 0].double() @ q[0, 0].double()), 0).max()) ** -1
+    tol = size * (2.0 ** -11 + 2.0 ** -12) + n * 2.0 ** -32 * float(v.abs().max()) / total \
+        + HALF_STEP[dtype] * ref.abs() * 1.01 + 2.0 ** -25
+    off = (out[:, 0].double() - ref).abs()
+    assert (off <= tol).all(), float((off / tol).max())
+    assert float(tol.max() / ref.abs().min()) < 0.05  # the bound is a bound
