@@ -51,6 +51,7 @@ constexpr int STEP = 32;                // tokens of a step
 // reference is set, and stays below 2^REACH, which fp16 holds.
 constexpr float HEAD = 7.f;
 constexpr float REACH = 15.f;
+constexpr float LARGE = 4194304.f;  // 2^22: half a 32-bit step is 1/4 log2 unit
 
 struct FewParams {
   AttnParams a;
@@ -155,6 +156,7 @@ template <int D, int NT>
 struct Acc {
   float o[D / 16][NT][4];  // O^T: channels n D/8 + 2t (+1), query rows 2c, 2c + 1 of tile nt
   float m[NT][2], l[NT][2];
+  bool large;  // some row of the warp has |m| > LARGE
 };
 
 // One step of 32 tokens (two blocks at `blk`): scores, running softmax, sums.
@@ -170,6 +172,11 @@ struct Acc {
 // 2^-21 of the largest are rounded to 2^-11 of themselves, smaller ones by 2^-32
 // of the largest at most (without HEAD 2^-25: a long context's small weights
 // beside one large one would count in l and be lost in O).
+//
+// m comes from a rounded product. Rows whose m is beyond LARGE round every score
+// as m was, or the largest would lie half a step of m off it, out of reach or out
+// of sight; the others take the difference unrounded. So equal keys weigh the
+// same whichever steps they are in.
 template <int D, int NT, bool MASK>
 __device__ __forceinline__ void step(Acc<D, NT>& acc, const uint8_t* blk, const uint8_t* sq, int lane,
                                      const float (&factor)[NT][2], int key0, int len, const int (&limit)[NT][2]) {
@@ -241,7 +248,8 @@ __device__ __forceinline__ void step(Acc<D, NT>& acc, const uint8_t* blk, const 
         y[b][nt][e] = hidden(b, nt, e) ? -INFINITY : fmaf(s[b][nt][e], factor[nt][e & 1], -acc.m[nt][e & 1]);
         far = fmaxf(far, y[b][nt][e]);
       }
-  if (__any_sync(0xffffffffu, far > REACH)) {
+  if (__any_sync(0xffffffffu, far > REACH) || acc.large) {
+    bool large = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -266,14 +274,19 @@ __device__ __forceinline__ void step(Acc<D, NT>& acc, const uint8_t* blk, const 
             acc.o[t][nt][2 + i] *= alpha;
           }
         }
-        // rounded as m was, so that the largest score comes within reach, however large
         const float m_use = acc.m[nt][i] == -INFINITY ? 0.f : acc.m[nt][i];
+        const bool rounded = fabsf(m_use) > LARGE;
+        large |= rounded;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int e = i; e < 4; e += 2)
-            y[b][nt][e] = hidden(b, nt, e) ? -INFINITY : __fsub_rn(__fmul_rn(s[b][nt][e], factor[nt][i]), m_use);
+          for (int e = i; e < 4; e += 2) {
+            const float x = rounded ? __fsub_rn(__fmul_rn(s[b][nt][e], factor[nt][i]), m_use)
+                                    : fmaf(s[b][nt][e], factor[nt][i], -m_use);
+            y[b][nt][e] = hidden(b, nt, e) ? -INFINITY : x;
+          }
       }
+    acc.large = __any_sync(0xffffffffu, large);
   }
   // P in fp16 (the sum keeps 32 bits), transposed into B fragments
   uint32_t pb[2][NT][2];
@@ -677,6 +690,7 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
         acc.m[nt][i] = -INFINITY;
         acc.l[nt][i] = 0.f;
       }
+    acc.large = false;
     least = a.causal ? min(len, len - tokens + 1 + a.token_of(row0)) : len;
 #pragma unroll
     for (int t = 0; t < D / 16; ++t)

@@ -62,3 +62,25 @@ def test_small_weights_beside_large_ones(nats, dtype, D, rows):
     off = (out[:, 0].double() - ref).abs()
     assert (off <= tol).all(), float((off / tol).max())
     assert float(tol.max() / ref.abs().min()) < 0.05  # the bound is a bound
+
+
+# 600 requests of one row over the same pages: pieces of all lengths; one request of many rows: the large kernel
+@pytest.mark.parametrize("requests,rows", [(600, 1), (1, 200)])
+@pytest.mark.parametrize("size", [8, 20, 23, 28, 60, 100])
+def test_equal_keys_weigh_the_same_however_large_their_scores(size, requests, rows):
+    """Two equal keys, in different steps, lead all others by far: the output is the mean of their values, which is
+    exact in 32 bits but for the weights' own rounding, the same for both; then one rounding of the output."""
+    n, D = 256, 64
+    k, v = torch.zeros(n, 1, D), torch.randn(n, 1, D, generator=torch.Generator().manual_seed(2))
+    k[3, 0, 0] = k[3 + 128, 0, 0] = 6.0
+    k[:, 0, 1] = -1.0
+    cache, table, k, v = held(k.half(), v.half())
+    q = torch.zeros(requests * rows, 1, D, dtype=torch.bfloat16)
+    q[:, 0, 0] = 2.0 ** size
+    args = (cache, table.expand(requests, -1).contiguous(), ints([n] * requests), ints(range(0, requests * rows + 1, rows)))
+    want = ((v[3, 0].double() + v[3 + 128, 0].double()) / 2).expand(requests * rows, -1)
+    for scale in (0.1, 0.77, 1 / 3):
+        out = g.attn_cache4(q.cuda(), *args, scale, causal=False, max_tokens=rows)[:, 0].cpu().double()
+        tol = HALF_STEP[torch.bfloat16] * 1.01 * want.abs() + 2.0 ** -20 * v.abs().max()
+        off = (out - want).abs()
+        assert (off <= tol).all(), (scale, float((off / tol).max()))
