@@ -198,7 +198,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) cache4_plan_kernel(const PlanPar
         position = len[lo] + t - start[lo];
         const int held = pages_of(len[lo]), at = position / PAGE;
         const int page = at < held ? p.tables[static_cast<long long>(lo) * p.width + at] : page_at(need[lo] + at - held);
-        slot = page * PAGE + position % PAGE;
+        // a slot has 31 bits: page ids that have none are no page of any cache
+        if (page >= 0 && page <= INT_MAX / PAGE) slot = page * PAGE + position % PAGE;
       }
     }
     p.slots[t] = slot;

@@ -39,7 +39,8 @@ GFX906_B200_API int gfx906_b200_cache4_page_bytes(int D);
  * at most 2^31 - 1;
  * lengths_out [requests]; added [requests], the tokens appended (0: refused or
  * ended); slots and positions [tokens], the slot and position of each token,
- * -1 for tokens of refused requests and behind the last; *free_count_out.
+ * -1 for tokens of refused requests and behind the last (the slot alone where
+ * the page id is negative or has no slots in 31 bits); *free_count_out.
  * tables and free_pages are updated in place, only in entries that the inputs
  * do not use, so a call may be repeated; the other outputs may not alias inputs. */
 GFX906_B200_API int gfx906_b200_cache4_plan(int* tables, const int* lengths, const int* counts, int* free_pages,

@@ -133,7 +133,9 @@ def plan(tables, lengths, counts, free_pages, free_count, tokens):
             for i in range(n):
                 at = lengths[r] + i
                 positions[start + i] = at
-                slots[start + i] = tables[r][at // PAGE] * PAGE + at % PAGE
+                page = tables[r][at // PAGE]
+                if 0 <= page <= (2 ** 31 - 1) // PAGE:  # else no slot has its number
+                    slots[start + i] = page * PAGE + at % PAGE
         added.append(n if ok else 0)
         new.append(0 if c < 0 else lengths[r] + added[-1])
     query_start = [min(n, 2 ** 31 - 1) for n in query_start]

@@ -84,3 +84,23 @@ def test_equal_keys_weigh_the_same_however_large_their_scores(size, requests, ro
         tol = HALF_STEP[torch.bfloat16] * 1.01 * want.abs() + 2.0 ** -20 * v.abs().max()
         off = (out - want).abs()
         assert (off <= tol).all(), (scale, float((off / tol).max()))
+
+
+@pytest.mark.parametrize("page", [-1, -2 ** 25 - 3, -2 ** 31, 2 ** 25, 2 ** 25 + 1, 2 ** 26 + 2, 2 ** 31 - 1])
+def test_plan_gives_no_slot_for_page_ids_beyond_slots(page):
+    """An id whose slots have no 31 bits must not come out as the slot of another page, granted or held already."""
+    held_by, free = [[page, 5, -1], [6, -1, -1]], [page, 9, page]
+    tables, free_pages = ints(held_by), ints(free)
+    plan = g.cache4_plan(tables, ints([64 + 60, 10]), ints([8, 64]), free_pages, ints([3]), 80)
+    want = oracle.plan(held_by, [64 + 60, 10], [8, 64], free, 3, 80)
+    assert plan.slots.tolist() == want["slots"] and plan.positions.tolist() == want["positions"]
+    assert plan.added.tolist() == [8, 64] and tables.tolist() == want["tables"]
+    # request 0: four tokens in page 5, four in the page granted first; request 1: 54 tokens in page 6, ten in page 9
+    assert want["slots"] == [5 * 64 + 60 + i for i in range(4)] + [-1] * 4 \
+        + [6 * 64 + 10 + i for i in range(54)] + [9 * 64 + i for i in range(10)] + [-1] * 8
+    plan = g.cache4_plan(ints([[page]]), ints([3]), ints([2]), free_pages, ints([0]), 2)
+    assert plan.slots.tolist() == [-1, -1] and plan.positions.tolist() == [3, 4]
+    k = torch.ones(2, 1, 64, dtype=torch.float16, device="cuda")
+    cache = g.cache4_alloc(4, 1, 64)
+    g.cache4_write(k, k, cache, plan.slots)
+    assert not cache.any()
