@@ -182,8 +182,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) cache4_plan_kernel(const PlanPar
       for (int i = lane; i < k; i += 32) row[held + i] = page_at(need[r] + i);
     }
   }
-  // tokens
-  for (int t = blockIdx.x * PLAN_THREADS + threadIdx.x; t < p.tokens; t += blocks * PLAN_THREADS) {
+  // tokens; a step behind the last one may leave 31 bits
+  for (unsigned next = blockIdx.x * PLAN_THREADS + threadIdx.x; next < static_cast<unsigned>(p.tokens);
+       next += blocks * PLAN_THREADS) {
+    const int t = static_cast<int>(next);
     int slot = -1, position = -1;
     if (t < total_tokens) {
       int lo = 0, hi = R - 1;  // last request that starts at or before t: the one that holds it

@@ -104,3 +104,14 @@ def test_plan_gives_no_slot_for_page_ids_beyond_slots(page):
     cache = g.cache4_alloc(4, 1, 64)
     g.cache4_write(k, k, cache, plan.slots)
     assert not cache.any()
+
+
+def test_plan_of_the_largest_token_buffer():
+    """Buffers near 2^31 tokens: every token behind the last is marked, none beyond the buffer is touched."""
+    tokens = 2 ** 31 - 2
+    plan = g.cache4_plan(ints([[0, 1]]), ints([3]), ints([5]), ints([2, 3]), ints([2]), tokens)
+    assert plan.slots[:6].tolist() == [3, 4, 5, 6, 7, -1] and plan.free_count.item() == 2
+    for x in (plan.slots, plan.positions):
+        assert x.shape == (tokens,) and int(x[5:].max()) == -1 and int(x[5:].min()) == -1
+    del plan, x
+    torch.cuda.empty_cache()
