@@ -850,7 +850,10 @@ static Plan plan_of(const gfx906_b200_cache4_attn_args& g, int sms) {
   pl.ml_off = slots * g.D * sizeof(float);
   pl.done_off = pl.ml_off + slots * 2 * sizeof(float);
   pl.many_off = (pl.done_off + pl.blocks * sizeof(unsigned long long) + 255) & ~static_cast<size_t>(255);
-  if (rows > FEW_ROWS) pl.many = many_plan(g.tokens, g.requests, g.heads / g.kv_heads, g.kv_heads, g.D, sms);
+  if (rows > FEW_ROWS && g.requests > 0) {
+    pl.many = many_plan(g.tokens, g.requests, g.heads / g.kv_heads, g.kv_heads, g.D, sms);
+    pl.fits = pl.fits && pl.many.fits;
+  }
   pl.bytes = pl.many_off + ((pl.many.bytes + 255) & ~static_cast<size_t>(255));
   return pl;
 }
@@ -880,8 +883,7 @@ static int attn(const gfx906_b200_cache4_attn_args& g, void* ws, size_t ws_bytes
   const int rc = gfx906_b200_internal_device(&sms);
   if (rc != GFX906_B200_OK) return rc;
   const Plan pl = plan_of(g, sms);
-  const bool any_many = static_cast<long long>(g.max_tokens) * (g.heads / g.kv_heads) > FEW_ROWS;
-  if (!pl.fits || (any_many && !pl.many.max_units)) return GFX906_B200_EINVAL;
+  if (!pl.fits) return GFX906_B200_EINVAL;
   if (!ws || ws_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(ws) & 255u)) return GFX906_B200_EINVAL;
   FewParams p{};
   p.a = {static_cast<const uint16_t*>(g.q), static_cast<uint16_t*>(g.o), static_cast<const uint8_t*>(g.cache), g.tables,
@@ -895,8 +897,6 @@ static int attn(const gfx906_b200_cache4_attn_args& g, void* ws, size_t ws_bytes
     ManyParams m{};
     m.a = p.a;
     m.min_rows = p.max_rows = FEW_ROWS;
-    m.max_units = pl.many.max_units;
-    m.sms = sms;
     m.max_units = pl.many.max_units;
     m.sms = sms;
     m.part_o = reinterpret_cast<float*>(base + pl.many_off);

@@ -851,6 +851,7 @@ ManyPlan many_plan(int tokens, int requests, int group, int kv_heads, int D, int
   ManyPlan pl{};
   const long long blocks = static_cast<long long>(tokens) * group / (2 * M_ROWS) + requests;
   if (blocks * kv_heads > INT_MAX / 1024 - sms * MAX_PIECES) return pl;
+  pl.fits = true;
   pl.max_units = static_cast<int>(blocks * kv_heads);
   // cut units: fewer than SMs
   const size_t rows = static_cast<size_t>(pl.max_units < sms ? pl.max_units : sms) * MAX_PIECES * 2 * M_ROWS;

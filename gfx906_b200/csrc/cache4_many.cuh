@@ -21,7 +21,8 @@ struct ManyParams {
   unsigned long long timeout_ns;
 };
 struct ManyPlan {
-  int max_units;  // 0: too large a call
+  bool fits;      // false: too large a call
+  int max_units;
   size_t ml_off, done_off, bytes;  // workspace
 };
 ManyPlan many_plan(int tokens, int requests, int group, int kv_heads, int D, int sms);

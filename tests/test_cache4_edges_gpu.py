@@ -115,3 +115,16 @@ def test_plan_of_the_largest_token_buffer():
         assert x.shape == (tokens,) and int(x[5:].max()) == -1 and int(x[5:].min()) == -1
     del plan, x
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("tokens", [1, 32, 33, 100, 127, 128, 300])
+def test_attention_without_requests(tokens):
+    """No request, a token buffer of any size: zeros, or `out` as it was."""
+    cache = g.cache4_alloc(2, 2, 64)
+    q = torch.ones(tokens, 4, 64, dtype=torch.float16, device="cuda")
+    for tables in (ints([]).reshape(0, 3), ints([]).reshape(0, 0)):
+        args = (cache, tables, ints([]), ints([0]), 0.1)
+        assert not g.attn_cache4(q, *args).any()
+        out = torch.full_like(q, 7.0)
+        g.attn_cache4(q, *args, out=out)
+        assert (out == 7).all()
