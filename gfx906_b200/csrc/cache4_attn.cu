@@ -10,7 +10,9 @@
 // end leaves partial sums (m, l, unnormalised O, 32 bits) in the workspace,
 // joined by the block that finishes its last piece. Every unit counts one step more than it has
 // keys for, so that units without any key have an owner that writes their
-// zeros, and as the price of starting a unit.
+// zeros, and as the price of starting a unit. Where tables are so wide that the
+// line could leave 31 bits, it counts grains of 2^k steps, a unit's last one
+// partly filled.
 //
 // Inside a block four warps take the steps in turn, each with its own ring of
 // copies in flight and its own running maximum m, sum l and accumulator; they
@@ -56,6 +58,7 @@ constexpr float LARGE = 4194304.f;  // 2^22: half a 32-bit step is 1/4 log2 unit
 struct FewParams {
   AttnParams a;
   int max_rows;       // requests with more query rows are another kernel's
+  int shift;          // a grain of the line is 2^shift steps
   float* part_o;      // [blocks][2][8 NT][D]
   float* part_ml;     // [blocks][2][8 NT][2]
   // [blocks] pieces in the workspace of the cut unit that the block starts,
@@ -138,17 +141,19 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return r;
 }
 
-// One request's part of the line of steps.
+// One request's part of the line.
 struct Share {
   int first, rows, len;  // first token; query rows (0: not this kernel's); keys
-  int units, steps;      // units; steps of one unit, with the one extra
+  int units, grains;     // units; grains of one unit's steps, with the one extra
 };
+__device__ __forceinline__ int steps_of(int len) { return (len + STEP - 1) / STEP + 1; }
 template <int ROWS>
 __device__ __forceinline__ Share share_of(const FewParams& p, int r) {
   const Rows t = rows_of(p.a, r);
   const int len = length_of(p.a, r), rows = t.n * p.a.group;
   if (rows > p.max_rows) return {t.first, 0, len, 0, 0};
-  return {t.first, rows, len, (rows + ROWS - 1) / ROWS * p.a.kv_heads, rows ? (len + STEP - 1) / STEP + 1 : 0};
+  return {t.first, rows, len, (rows + ROWS - 1) / ROWS * p.a.kv_heads,
+          rows ? (steps_of(len) + (1 << p.shift) - 1) >> p.shift : 0};
 }
 
 // Per-thread state of one warp's share of a unit.
@@ -338,14 +343,14 @@ __device__ __forceinline__ void step(Acc<D, NT>& acc, const uint8_t* blk, const 
   }
 }
 
-// The line of `total` steps in `blocks` runs: run c starts at total * c / blocks,
+// The line of `total` grains in `blocks` runs: run c starts at total * c / blocks,
 // so that equal units which the blocks divide evenly are cut where they end.
 struct Split {
   int total, blocks, per, more;
   __device__ __forceinline__ Split(int total_, int blocks_)
       : total(total_), blocks(blocks_), per(total_ / blocks_), more(total_ - per * blocks_) {}
   __device__ __forceinline__ int start(int c) const { return c * per + c * more / blocks; }
-  // the run that holds step `at`
+  // the run that holds grain `at`
   __device__ __forceinline__ int owner(int at) const {
     int c = min(blocks - 1, static_cast<int>(static_cast<float>(at) * blocks / total));  // off by one or two
     while (c > 0 && start(c) > at) --c;
@@ -493,7 +498,7 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
   fa::griddep_wait();
   if (threadIdx.x == 0) fa::griddep_launch_dependents();
 
-  // ---- this block's part [pos, end) of the line of steps
+  // ---- this block's part [pos, end) of the line
   const int chunks = (a.requests + THREADS - 1) / THREADS;
   long long total64 = 0;
   int units = 0;
@@ -504,7 +509,7 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
     if (r < a.requests) mine = share_of<C::ROWS>(p, r);
     // a request's weight fits 31 bits (the host sees to it), their sum may not,
     // if query_start decreases somewhere: it is added up in two halves
-    const unsigned weight = static_cast<unsigned>(mine.units) * mine.steps;
+    const unsigned weight = static_cast<unsigned>(mine.units) * mine.grains;
     const unsigned low = __reduce_add_sync(0xffffffffu, weight & 0xffffu);
     const unsigned high = __reduce_add_sync(0xffffffffu, weight >> 16);
     const unsigned u = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(mine.units));
@@ -527,7 +532,8 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
   // as many blocks as there are, or as many for each unit as its steps are
   // worth: equal units are then cut into equal pieces, or not at all
   int blocks = gridDim.x;
-  if (total < blocks * C::MIN_STEPS) blocks = total ? min(blocks, units * max(1, total / units / C::MIN_STEPS)) : 0;
+  const int least_run = max(1, C::MIN_STEPS >> p.shift);
+  if (total < blocks * least_run) blocks = total ? min(blocks, units * max(1, total / units / least_run)) : 0;
   const Split split(total, max(blocks, 1));
   int pos = 0, end = 0;
   if (static_cast<int>(blockIdx.x) < blocks) {
@@ -541,7 +547,7 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
     while (k + 1 < chunks && chunk_before[k + 1] <= pos) ++k;
     r = k * THREADS + threadIdx.x;
     if (chunks > 1) mine = r < a.requests ? share_of<C::ROWS>(p, r) : Share{};
-    const int w = mine.units * mine.steps;
+    const int w = mine.units * mine.grains;
     int inc = w;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
@@ -564,22 +570,23 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
   }
 
   while (pos < end) {
-    if (pos - base >= sh.units * sh.steps) {  // the next request (the line ends with the last one's units)
-      base += sh.units * sh.steps;
+    if (pos - base >= sh.units * sh.grains) {  // the next request (the line ends with the last one's units)
+      base += sh.units * sh.grains;
       ++r;
       sh = share_of<C::ROWS>(p, r);
       continue;
     }
-    const int unit = (pos - base) / sh.steps;
-    const int off = pos - base - unit * sh.steps;
-    const int stop = min(sh.steps, off + end - pos);
+    const int unit = (pos - base) / sh.grains;
+    const int off = pos - base - unit * sh.grains;
+    const int stop = min(sh.grains, off + end - pos);
     const int head = unit % a.kv_heads;
     const int row0 = unit / a.kv_heads * C::ROWS;
     const int nrows = min(C::ROWS, sh.rows - row0);
     const int len = sh.len, tokens = a.token_of(sh.rows);
-    const int k_begin = max(off, 1) - 1, k_end = stop - 1;  // steps that hold keys
+    // steps that hold keys
+    const int k_begin = max(off << p.shift, 1) - 1, k_end = min(stop << p.shift, steps_of(len)) - 1;
     const int* table = a.tables + static_cast<long long>(r) * a.width;
-    const bool starts = off == 0, ends = stop == sh.steps;
+    const bool starts = off == 0, ends = stop == sh.grains;
     const int first_block = starts ? static_cast<int>(blockIdx.x) : split.owner(pos - off);
     const float kf = a.scale_log2 * (a.k_scale ? a.k_scale[head] : 1.f);
     const float vf = a.v_scale ? a.v_scale[head] : 1.f;
@@ -790,7 +797,7 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
       // thread 0's fence, and that before its count.
       __syncthreads();
       if (threadIdx.x == 0) {
-        const int pieces = split.owner(pos - off + sh.steps - 1) - first_block + 1;
+        const int pieces = split.owner(pos - off + sh.grains - 1) - first_block + 1;
         __threadfence();
         const int before = static_cast<int>(atomicAdd(count, 1ull) & 0xffffull);
         joins = before + 1 == pieces;
@@ -802,7 +809,7 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
       __syncthreads();
       if (joins)
         join<D, NT, BF16>(p, reinterpret_cast<float*>(smem), first_block,
-                          split.owner(pos - off + sh.steps - 1) - first_block + 1, sh.first, row0, nrows, head, vf);
+                          split.owner(pos - off + sh.grains - 1) - first_block + 1, sh.first, row0, nrows, head, vf);
     }
     pos += stop - off;
     fa::fence_proxy_async_smem();  // what was stored in the rings comes before the next copies
@@ -830,6 +837,7 @@ static bool args_ok(const gfx906_b200_cache4_attn_args& g) {
 struct Plan {
   int nt;      // row tiles of 8 NT rows
   int blocks;
+  int shift;   // grains of the line
   size_t ml_off, done_off, many_off, bytes;
   bool fits;
   ManyPlan many;  // max_units 0: no request has that many rows
@@ -839,12 +847,15 @@ static Plan plan_of(const gfx906_b200_cache4_attn_args& g, int sms) {
   const long long rows = static_cast<long long>(g.max_tokens) * (g.heads / g.kv_heads);
   pl.nt = rows <= 8 ? 1 : 2;
   pl.blocks = sms * (pl.nt == 1 ? Few<128, 1>::PER_SM : Few<128, 2>::PER_SM);
-  // the line of steps is counted in 31 bits
+  // the line is counted in 31 bits: in single steps, unless the tables could hold
+  // more of them (the lengths are not known here)
   const long long tiles = rows > FEW_ROWS ? static_cast<long long>(g.requests) * (FEW_ROWS / (8 * pl.nt))
                                           : static_cast<long long>(g.tokens) * (g.heads / g.kv_heads) / (8 * pl.nt) + g.requests;
-  pl.fits = tiles * g.kv_heads <= INT_MAX / (2ll * g.width + 2);
+  const long long units = tiles * g.kv_heads, steps = 2ll * g.width + 1;
+  pl.fits = units <= INT_MAX;
+  while (pl.fits && units * (((steps - 1) >> pl.shift) + 1) > INT_MAX) ++pl.shift;
   // no more blocks than the tables can hold steps for
-  const long long most = pl.fits ? tiles * g.kv_heads * max(1ll, (2ll * g.width + 1) / Few<128, 1>::MIN_STEPS) : 1;
+  const long long most = pl.fits ? units * max(1ll, steps / Few<128, 1>::MIN_STEPS) : 1;
   pl.blocks = static_cast<int>(min(static_cast<long long>(pl.blocks), max(1ll, most)));
   const size_t slots = static_cast<size_t>(pl.blocks) * 2 * 8 * pl.nt;
   pl.ml_off = slots * g.D * sizeof(float);
@@ -892,6 +903,7 @@ static int attn(const gfx906_b200_cache4_attn_args& g, void* ws, size_t ws_bytes
          g.scale * 1.4426950408889634f,
          group_magic(static_cast<long long>(g.tokens) * (g.heads / g.kv_heads), g.heads / g.kv_heads)};
   p.max_rows = INT_MAX;
+  p.shift = pl.shift;
   uint8_t* base = static_cast<uint8_t*>(ws);
   if (pl.many.max_units > 0) {
     ManyParams m{};

@@ -850,7 +850,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
 ManyPlan many_plan(int tokens, int requests, int group, int kv_heads, int D, int sms) {
   ManyPlan pl{};
   const long long blocks = static_cast<long long>(tokens) * group / (2 * M_ROWS) + requests;
-  if (blocks * kv_heads > INT_MAX / 1024 - sms * MAX_PIECES) return pl;
+  if (blocks * kv_heads > INT_MAX - CUT_CTAS * sms) return pl;  // CTAs of a launch
   pl.fits = true;
   pl.max_units = static_cast<int>(blocks * kv_heads);
   // cut units: fewer than SMs

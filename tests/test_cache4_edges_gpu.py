@@ -128,3 +128,44 @@ def test_attention_without_requests(tokens):
         out = torch.full_like(q, 7.0)
         g.attn_cache4(q, *args, out=out)
         assert (out == 7).all()
+
+
+def check_rows(out, q, k, v, scale, causal, rows, heads, group):
+    """Rows of one request of n = len(out) tokens: p's rounding and 32-bit scores, and one rounding of the output."""
+    n, length = len(out), len(k)
+    for i in rows:
+        last = length - n + i + 1 if causal else length
+        for h in heads:
+            ref, size = oracle.attention(q[i, h][None], k[:last, h // group], v[:last, h // group], scale, False)
+            tol = size * (2.0 ** -11 + 2.0 ** -12) + HALF_STEP[out.dtype] * ref.abs() * 1.01 \
+                + last * 2.0 ** -32 * float(v.abs().max()) + 2.0 ** -25
+            off = (out[i, h].cpu().double() - ref[0]).abs()
+            assert (off <= tol[0]).all(), (i, h, float((off / tol[0]).max()))
+
+
+@pytest.mark.parametrize("rows,length", [(1, 5000), (1, 31), (13, 1999), (60, 700)])
+def test_attention_with_the_widest_table(rows, length):
+    """A table of 2^25 - 1 pages, of which few are used: the call's size is that of the lengths."""
+    H, D, width = 32, 64, 2 ** 25 - 1
+    gen = torch.Generator().manual_seed(4)
+    cache, table, k, v = held(*(torch.randn(length, H, D, generator=gen).half() for _ in range(2)))
+    wide = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    q = torch.randn(rows, H, D, generator=gen).half()
+    out = g.attn_cache4(q.cuda(), cache, wide, ints([length]), ints([0, rows]), 0.125, max_tokens=rows)
+    check_rows(out, q, k, v, 0.125, True, range(0, rows, 7), [0, 1, 30, 31], 1)
+
+
+@pytest.mark.parametrize("hint", [None, 1])
+def test_attention_of_many_requests_with_wide_tables(hint):
+    """4096 requests, 32 heads, room for 131072 tokens each."""
+    R, H, D, width = 4096, 32, 64, 2048
+    gen = torch.Generator().manual_seed(5)
+    cache, table, k, v = held(*(torch.randn(300, H, D, generator=gen).half() for _ in range(2)))
+    tables = torch.full((R, width), -1, dtype=torch.int32, device="cuda")
+    tables[:, :table.shape[1]] = table
+    lengths = [1 + 37 * r % 300 for r in range(R)]
+    q = torch.randn(R, H, D, generator=gen).half()
+    out = g.attn_cache4(q.cuda(), cache, tables, ints(lengths), ints(range(R + 1)), 0.125, max_tokens=hint)
+    for r in (0, 1, 63, 64, 1000, 4095):
+        check_rows(out[r:r + 1], q[r:r + 1], k[:lengths[r]], v[:lengths[r]], 0.125, True, [0], [0, 13, 31], 1)
