@@ -821,10 +821,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
           unsigned long long* count = p.done + sg.tail * 2 + at.tile;
           __threadfence();
           const bool last = static_cast<int>(atomicAdd(count, 1ull) & 0xffffull) + 1 == sg.pieces;
-          if (last) {
-            __threadfence();
-            atomicExch(count, p.epoch << 16);
-          }
+          if (last) __threadfence();
           last_flag[at.tile] = last;
         }
         mbar_arrive(bar + 8 * C::B_WG);
@@ -857,7 +854,8 @@ ManyPlan many_plan(int tokens, int requests, int group, int kv_heads, int D, int
   const size_t rows = static_cast<size_t>(pl.max_units < sms ? pl.max_units : sms) * MAX_PIECES * 2 * M_ROWS;
   pl.ml_off = rows * D * sizeof(float);
   pl.done_off = pl.ml_off + rows * 2 * sizeof(float);
-  pl.bytes = pl.done_off + static_cast<size_t>(sms) * 2 * sizeof(unsigned long long);
+  pl.done_words = sms * 2;
+  pl.bytes = pl.done_off + pl.done_words * sizeof(unsigned long long);
   return pl;
 }
 

@@ -1,9 +1,13 @@
 """The paged 4-bit cache at the edges of its numbers, sizes and memory (needs a B200)."""
 
+import ctypes
+
 import pytest
 import torch
 
 import gfx906_b200 as g
+from gfx906_b200 import build
+from gfx906_b200.cabi import CABI, STATUS, Cache4AttnArgs
 from oracle import cache4 as oracle
 
 pytestmark = pytest.mark.gpu
@@ -169,3 +173,43 @@ def test_attention_of_many_requests_with_wide_tables(hint):
     out = g.attn_cache4(q.cuda(), cache, tables, ints(lengths), ints(range(R + 1)), 0.125, max_tokens=hint)
     for r in (0, 1, 63, 64, 1000, 4095):
         check_rows(out[r:r + 1], q[r:r + 1], k[:lengths[r]], v[:lengths[r]], 0.125, True, [0], [0, 13, 31], 1)
+
+
+def c_call(q, out, cache, tables, lengths, query_start, scale, causal=True):
+    """(run, workspace) of one attention call through the C ABI on the current stream, which `run` launches."""
+    lib = CABI(build.LIB_PATH)
+    a = Cache4AttnArgs(q=q.data_ptr(), o=out.data_ptr(), cache=cache.data_ptr(), tables=tables.data_ptr(),
+                       lengths=lengths.data_ptr(), query_start=query_start.data_ptr(), q_stride_t=q.stride(0),
+                       q_stride_h=q.stride(1), o_stride_t=out.stride(0), o_stride_h=out.stride(1),
+                       dtype=int(q.dtype == torch.bfloat16), tokens=q.shape[0], heads=q.shape[1],
+                       kv_heads=cache.shape[1], D=q.shape[2], pages=cache.shape[0], requests=tables.shape[0],
+                       width=tables.shape[1], max_tokens=q.shape[0], causal=int(causal), zero_rest=1, scale=scale)
+    ws = torch.empty(lib.dll.gfx906_b200_cache4_attn_workspace_size(ctypes.byref(a)), dtype=torch.uint8, device="cuda")
+
+    def run():
+        rc = lib.dll.gfx906_b200_cache4_attn(ctypes.byref(a), ws.data_ptr(), ws.numel(),
+                                             torch.cuda.current_stream().cuda_stream)
+        assert rc == STATUS["OK"]
+    return run, ws
+
+
+def test_no_count_of_a_launch_is_left_for_its_replay():
+    """Pieces of many rows are counted in the workspace's last words under the launch's tag, which a replayed graph
+    keeps. A CTA whose wait runs out does not count; were a partial count left, every replay would join too early."""
+    n, rows, gen = 4500, 600, torch.Generator().manual_seed(6)
+    cache, table, k, v = held(*(torch.randn(n, 1, 64, generator=gen).half() for _ in range(2)))
+    q = torch.randn(rows, 1, 64, generator=gen).half().cuda()
+    args = (cache, table, ints([n]), ints([0, rows]), 0.125)
+    want, out = g.attn_cache4(q, *args), torch.empty_like(q)
+    run, ws = c_call(q, out, *args)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    words = ws[-(-(-16 * sms // 256) * 256):].view(torch.int64)[:2 * sms]  # two to an SM, the region a multiple of 256 bytes
+    ws.fill_(0x5a)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for _ in range(3):
+        out.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and not words.any()
