@@ -49,6 +49,7 @@ constexpr int FEW_ROWS = 64;
 
 constexpr int MAX_REQUESTS = 8192;
 constexpr int STEP = 32;                // tokens of a step
+constexpr unsigned long long DRAIN_NS = 100000000ull;  // see the kernel's waits
 // Log2 units, see step(): P of a row's largest score is 2^HEAD when the row's
 // reference is set, and stays below 2^REACH, which fp16 holds.
 constexpr float HEAD = 7.f;
@@ -614,7 +615,7 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
     // ---- copies of this warp's first steps
     int page_ids = 0, ids_at = -32;  // page of step k_begin + warp + WARPS * (ids_at + lane)
     const int my_steps = k_end - k_begin - warp > 0 ? (k_end - k_begin - warp + WARPS - 1) / WARPS : 0;
-    uint32_t good = 0;  // bit: the step in that stage has a page
+    uint32_t good = 0;  // bit: that stage holds or awaits a step whose page is in the cache
     int issued = 0;
     auto issue = [&]() {
       if (issued < my_steps && !late) {
@@ -719,6 +720,7 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
           break;
         }
         phases ^= 1u << stage;
+        good &= ~(1u << stage);
         const int key0 = (k_begin + warp + WARPS * i) * STEP;
         if (key0 + STEP > least)
           step<D, NT, true>(acc, ring_at + stage * C::STEP_BYTES, smem + C::Q_OFF, lane, factor, key0, len, limit);
@@ -728,10 +730,12 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
       __syncwarp();  // the stage is free for the next copy
     }
     // a copy that did not come in time: the status word is set, this warp takes no
-    // further steps, and waits (for as long again) until none is in flight
+    // further steps, and waits until none is in flight (at least DRAIN_NS for each,
+    // however short the limit: what lands after the block's end lands in another's memory)
     if (late) {
       for (int stage = 0; stage < C::STAGES; ++stage)
-        if ((good >> stage) & 1u) wait_copy(copied + 8 * stage, (phases >> stage) & 1u, p.timeout_ns);
+        if ((good >> stage) & 1u)
+          wait_copy(copied + 8 * stage, (phases >> stage) & 1u, p.timeout_ns > DRAIN_NS ? p.timeout_ns : DRAIN_NS);
     }
 
     // ---- the four warps' sums become one
