@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
     const int len = length_of(a, u.r), row0 = u.block * 2 * M_ROWS;
     const int last_token = a.token_of(min(rows.n * a.group, row0 + 2 * M_ROWS) - 1);
     const int seen = a.causal ? max(0, min(len, len - rows.n + 1 + last_token)) : len;
-    const int tiles = (seen + BN - 1) / BN;
+    const int tiles = static_cast<int>((static_cast<unsigned>(seen) + BN - 1) / BN);
     const int pieces = max(1, min(u.most, tiles / MIN_TILES));
     if (u.piece >= pieces) return;
     if (threadIdx.x == 0) {

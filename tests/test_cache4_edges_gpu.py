@@ -240,3 +240,17 @@ def test_attention_under_the_shortest_wait_limit():
     got = subprocess.run([sys.executable, "-c", SHORT_WAITS], capture_output=True, text=True, timeout=120,
                          cwd=build.PKG_DIR.parent, env={**os.environ, "GFX906_B200_WAIT_TIMEOUT_MS": "1"})
     assert got.returncode == 0 and "done" in got.stdout, got.stderr
+
+
+@pytest.mark.parametrize("rows", [1, 65])
+def test_attention_to_the_longest_context(rows):
+    """2^31 - 64 tokens, the most that a table can hold: all in one page but for the last 64, which outweigh them."""
+    k, v = torch.zeros(128, 1, 64), torch.ones(128, 1, 64)
+    k[64:, 0, 0], v[64:] = 6.0, 3.0
+    cache, _, k, v = held(k.half(), v.half())
+    tables = torch.zeros(1, 2 ** 25 - 1, dtype=torch.int32, device="cuda")
+    tables[0, -1] = 1
+    q = torch.zeros(rows, 1, 64, dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 20.0
+    out = g.attn_cache4(q, cache, tables, ints([2 ** 31 - 64]), ints([0, rows]), 0.5, causal=False, max_tokens=rows)
+    assert (out == float(v[64, 0, 0])).all()  # the others weigh 2^31 e^-60 together
