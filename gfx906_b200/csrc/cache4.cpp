@@ -53,16 +53,20 @@ int dtype_code(const Tensor& t, const char* name) {
   return t.dtype() == torch::kBFloat16 ? 1 : 0;
 }
 
+// Elements from one token (dim 0) or head (dim 1) to the next. A dimension of one
+// entry may have any stride in torch; no kernel uses it.
+int64_t stride_of(const Tensor& t, int dim) { return t.size(dim) == 1 ? t.size(2) : t.stride(dim); }
+
 // Rows the kernels can load 16 bytes at a time: contiguous in the head dim,
 // starting on 16 bytes. Anything else is copied once.
 bool rows_ok(const Tensor& t) {
-  return (t.size(2) == 1 || t.stride(2) == 1) && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+  return t.stride(2) == 1 && stride_of(t, 0) % 8 == 0 && stride_of(t, 1) % 8 == 0 &&
          reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 Tensor with_rows(const Tensor& t) {
   if (t.numel() == 0 || rows_ok(t)) return t;
-  Tensor c = t.contiguous();
-  return rows_ok(c) ? c : c.clone();  // a contiguous view may start off 16 bytes
+  // a contiguous view may start off 16 bytes
+  return t.is_contiguous() ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous();
 }
 
 // These calls are as short as their launches, so results are allocated without
@@ -144,9 +148,10 @@ void cache4_write(Tensor k, Tensor v, Tensor cache, Tensor slots, std::optional<
   const float* vs = check_scale(v_scale, cache, heads, "v_scale");
   const c10::cuda::CUDAGuard guard(cache.device());
   const Tensor kc = with_rows(k), vc = with_rows(v);
-  check_status(gfx906_b200_cache4_write(kc.data_ptr(), vc.data_ptr(), dtype, kc.stride(0), kc.stride(1), vc.stride(0),
-                                        vc.stride(1), static_cast<int>(k.size(0)), heads, D, cache.data_ptr(), pages,
-                                        slots.data_ptr<int>(), ks, vs, at::cuda::getCurrentCUDAStream()));
+  check_status(gfx906_b200_cache4_write(kc.data_ptr(), vc.data_ptr(), dtype, stride_of(kc, 0), stride_of(kc, 1),
+                                        stride_of(vc, 0), stride_of(vc, 1), static_cast<int>(k.size(0)), heads, D,
+                                        cache.data_ptr(), pages, slots.data_ptr<int>(), ks, vs,
+                                        at::cuda::getCurrentCUDAStream()));
 }
 
 std::tuple<Tensor, Tensor> cache4_read(Tensor cache, Tensor slots, std::optional<Tensor> k_scale,
@@ -203,10 +208,10 @@ Tensor attn_cache4(Tensor q, Tensor cache, Tensor tables, Tensor lengths, Tensor
   g.query_start = query_start.data_ptr<int>();
   g.k_scale = ks;
   g.v_scale = vs;
-  g.q_stride_t = qc.stride(0);
-  g.q_stride_h = qc.stride(1);
-  g.o_stride_t = o.stride(0);
-  g.o_stride_h = o.stride(1);
+  g.q_stride_t = stride_of(qc, 0);
+  g.q_stride_h = stride_of(qc, 1);
+  g.o_stride_t = stride_of(o, 0);
+  g.o_stride_h = stride_of(o, 1);
   g.dtype = dtype;
   g.tokens = static_cast<int>(q.size(0));
   g.heads = static_cast<int>(q.size(1));

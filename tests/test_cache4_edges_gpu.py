@@ -254,3 +254,31 @@ def test_attention_to_the_longest_context(rows):
     q[:, :, 0] = 20.0
     out = g.attn_cache4(q, cache, tables, ints([2 ** 31 - 64]), ints([0, rows]), 0.5, causal=False, max_tokens=rows)
     assert (out == float(v[64, 0, 0])).all()  # the others weigh 2^31 e^-60 together
+
+
+@pytest.mark.parametrize("tokens,heads", [(5, 1), (1, 3), (1, 1)])
+def test_dimensions_of_one_entry_may_have_any_stride(tokens, heads):
+    gen = torch.Generator().manual_seed(7)
+    plain = [torch.randn(tokens, heads, 64, generator=gen).half().cuda() for _ in range(3)]
+    if heads == 1:  # [tokens, 64, 1] seen as [tokens, 1, 64]: a stride of one from head to head
+        odd = [x.transpose(1, 2).contiguous().transpose(1, 2).as_strided((tokens, 1, 64), (64, 1, 1)) for x in plain]
+    else:  # [heads, 64, 1] seen as [1, heads, 64]: a stride of one from token to token
+        odd = [x.as_strided((1, heads, 64), (1, 64, 1)) for x in plain]
+    late = []  # the same, starting off 16 bytes
+    for x in odd:
+        y = torch.empty(x.numel() + 1, dtype=x.dtype, device="cuda")[1:].as_strided(x.shape, x.stride())
+        late.append(y.copy_(x))
+    slots, tables = ints(range(tokens)), ints([[0]])
+    want = g.cache4_alloc(1, heads, 64)
+    g.cache4_write(plain[0], plain[1], want, slots)
+    args = (tables, ints([tokens]), ints([0, tokens]), 0.2)
+    o = g.attn_cache4(plain[2], want, *args)
+    for k, v, q in (odd, late):
+        assert k.is_contiguous() and 1 in k.stride()[:2]
+        cache = g.cache4_alloc(1, heads, 64)
+        g.cache4_write(k, v, cache, slots)
+        assert torch.equal(cache, want)
+        assert torch.equal(g.attn_cache4(q, cache, *args), o)
+    out = torch.zeros_like(o).as_strided(odd[2].shape, odd[2].stride())
+    g.attn_cache4(odd[2], want, *args, out=out)
+    assert torch.equal(out, o)
