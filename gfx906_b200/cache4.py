@@ -138,7 +138,8 @@ def attn_cache4(q, cache, tables, lengths, query_start, scale, causal=True, k_sc
     kernels (default: all rows of q may be one request's). Too small a value
     costs time, not correctness. Returns a new tensor, with zeros in rows behind
     the last request, or ``out``, whose rows behind the last request are left
-    as they were.
+    as they were. ``out`` is q itself, or shares no row with q and no memory
+    with the other arguments.
     """
     return _module().attn_cache4(q, cache, tables, lengths, query_start, float(scale), bool(causal), k_scale, v_scale,
                                  max_tokens, out)

@@ -2,15 +2,16 @@
 // (include/gfx906_b200_cache4.h). Like `attn`: inputs are checked, launched on
 // the current stream of their device, and failures raise RuntimeError.
 #include <torch/extension.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <algorithm>
 #include <optional>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "../../include/gfx906_b200_cache4.h"
 
@@ -67,6 +68,52 @@ Tensor with_rows(const Tensor& t) {
   if (t.numel() == 0 || rows_ok(t)) return t;
   // a contiguous view may start off 16 bytes
   return t.is_contiguous() ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous();
+}
+
+// Where the rows [tokens, heads] of a tensor start, in elements.
+struct RowGrid {
+  int64_t at, step_t, step_h;
+  explicit RowGrid(const Tensor& t)
+      : at(reinterpret_cast<intptr_t>(t.data_ptr()) / 2), step_t(stride_of(t, 0)), step_h(stride_of(t, 1)) {}
+};
+// Do two different rows of D elements of one grid share an element? Of two rows
+// dh >= 0 heads apart the nearest are those whose distance in tokens makes up for it.
+bool rows_meet(const RowGrid& a, int64_t T, int64_t H, int64_t D, int64_t offset, bool same) {
+  for (int64_t dh = same ? 0 : 1 - H; dh < H; ++dh) {
+    const int64_t far = offset + dh * a.step_h;
+    if (same && dh == 0) {
+      if (T > 1 && a.step_t < D) return true;
+      continue;
+    }
+    const int64_t near = a.step_t ? -far / a.step_t : 0;
+    for (int64_t dt = near - 1; dt <= near + 1; ++dt)
+      if (std::abs(dt) < T && std::abs(far + dt * a.step_t) < D) return true;
+  }
+  return false;
+}
+// Rows of out that are not its own, or that are rows of q other than the same ones:
+// calls write rows while others are still read.
+bool out_ok(const Tensor& out, const Tensor& q) {
+  const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
+  if (q.numel() == 0) return true;
+  const RowGrid o(out), x(q);
+  if (!(o.step_h >= D && o.step_t >= (H - 1) * o.step_h + D) && rows_meet(o, T, H, D, 0, true)) return false;
+  const auto end = [&](const RowGrid& g) { return g.at + (T - 1) * g.step_t + (H - 1) * g.step_h + D; };
+  if (o.at >= end(x) || x.at >= end(o)) return true;
+  if (o.step_t == x.step_t && o.step_h == x.step_h) return o.at == x.at || !rows_meet(o, T, H, D, o.at - x.at, false);
+  // two orders in one piece of memory: every row of one against its neighbours in the other
+  std::vector<int64_t> rows;
+  rows.reserve(T * H);
+  for (int64_t t = 0; t < T; ++t)
+    for (int64_t h = 0; h < H; ++h) rows.push_back(x.at + t * x.step_t + h * x.step_h);
+  std::sort(rows.begin(), rows.end());
+  for (int64_t t = 0; t < T; ++t)
+    for (int64_t h = 0; h < H; ++h) {
+      const int64_t row = o.at + t * o.step_t + h * o.step_h;
+      const auto next = std::upper_bound(rows.begin(), rows.end(), row - D);
+      if (next != rows.end() && *next < row + D) return false;
+    }
+  return true;
 }
 
 // These calls are as short as their launches, so results are allocated without
@@ -191,12 +238,14 @@ Tensor attn_cache4(Tensor q, Tensor cache, Tensor tables, Tensor lengths, Tensor
   TORCH_CHECK(!max_tokens.has_value() || *max_tokens >= 0, "cache4: max_tokens must not be negative");
   const float* ks = check_scale(k_scale, cache, kv_heads, "k_scale");
   const float* vs = check_scale(v_scale, cache, kv_heads, "v_scale");
-  if (out.has_value())
+  if (out.has_value()) {
     TORCH_CHECK(out->is_cuda() && out->device() == q.device() && out->dtype() == q.dtype() && out->sizes() == q.sizes() &&
-                    rows_ok(*out) && at::has_internal_overlap(*out) != at::MemOverlap::Yes,
-                "cache4: out must be a tensor like q with rows of its own that start on 16 bytes");
+                    rows_ok(*out),
+                "cache4: out must be a tensor like q with rows that start on 16 bytes");
+  }
   const c10::cuda::CUDAGuard guard(cache.device());
   const Tensor qc = with_rows(q);
+  TORCH_CHECK(!out.has_value() || out_ok(*out, qc), "cache4: out must have rows of its own: q itself, or no row of q");
   Tensor o = out.has_value() ? *out : new_tensor(q.sizes(), q.scalar_type(), q);
   if (q.numel() == 0) return o;
   gfx906_b200_cache4_attn_args g{};

@@ -282,3 +282,50 @@ def test_dimensions_of_one_entry_may_have_any_stride(tokens, heads):
     out = torch.zeros_like(o).as_strided(odd[2].shape, odd[2].stride())
     g.attn_cache4(odd[2], want, *args, out=out)
     assert torch.equal(out, o)
+
+
+def test_out_shares_no_row_with_other_rows_of_q():
+    T, H, D, gen = 6, 6, 64, torch.Generator().manual_seed(8)
+    cache, table, _, _ = held(*(torch.randn(300, H, D, generator=gen).half() for _ in range(2)))
+    q = torch.randn(T, H, D, generator=gen).half().cuda()
+    args = (cache, table, ints([300]), ints([0, T]), 0.2)
+    want = g.attn_cache4(q, *args)
+    row = H * D
+    memory = torch.empty(4 * T * row, dtype=torch.float16, device="cuda")
+
+    def view(at, step_t, step_h):
+        return memory.as_strided((T, H, D), (step_t, step_h, 1), at)
+
+    fine = [(view(0, row, D), view(0, row, D)),                       # in place
+            (view(0, row, D), view(T * row, row, D)),                 # one behind the other
+            (view(row, 3 * row, D), view(0, 3 * row, D)),             # parts of a fused projection
+            (view(0, 2 * row, 2 * D), view(D, 2 * row, 2 * D)),       # head by head
+            (view(0, D, T * D), view(T * row, row, D)),               # two orders, apart
+            (view(0, 2 * row, D), view(row, D, 2 * row)),             # two orders, interleaved
+            (view(0, 4 * row, D), view(row + 8, 4 * row, D))]
+    for x, out in fine:
+        memory.zero_()
+        x.copy_(q)
+        g.attn_cache4(x, *args, out=out)
+        assert torch.equal(out, want)
+    bad = [(view(0, row, D), view(row, row, D)),                      # one token on
+           (view(row, row, D), view(0, row, D)),
+           (view(0, row, D), view(D, row, D)),                        # one head on
+           (view(0, row, D), view(8, row, D)),                        # a part of a row
+           (view(0, row, D), view((T - 1) * row + (H - 1) * D, row, D)),  # the last row alone
+           (view(0, row, D), view(0, D, T * D)),                      # the same rows in another order
+           (view(0, row, D), view(0, 2 * row, D)),
+           (view(0, 2 * row, D), view(row - 8, D, 2 * row)),
+           (view(0, row, D), view(3 * T * row // 2, D, D)),           # rows of out on top of each other
+           (view(0, row, D), view(3 * T * row // 2, 0, D)),
+           (view(0, row, D), view(3 * T * row // 2, 5 * D, D)),
+           (view(0, row, D), view(3 * T * row // 2, D, 8))]
+    for x, out in bad:
+        with pytest.raises(RuntimeError, match="rows of its own"):
+            g.attn_cache4(x, *args, out=out)
+    # rows that the kernels cannot load are copied first, and out may be where they were
+    spread = memory[:T * row * 2].view(T, H, D, 2)[..., 0]
+    spread.copy_(q)
+    out = view(0, row, D)
+    g.attn_cache4(spread, *args, out=out)
+    assert torch.equal(out, want)
