@@ -49,7 +49,7 @@ _READ_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
 class Cache4Plan(NamedTuple):
-    """What ``cache4_plan`` found for a step (int32 CUDA tensors)."""
+    """What ``cache4_plan`` found for a step: int32 CUDA tensors, parts of one allocation."""
 
     query_start: torch.Tensor  # [requests + 1] first token of each request in the packed batch, and their sum
     lengths: torch.Tensor      # [requests] tokens in the cache once the new ones are written

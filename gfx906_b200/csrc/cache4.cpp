@@ -117,7 +117,7 @@ bool out_ok(const Tensor& out, const Tensor& q) {
 }
 
 // These calls are as short as their launches, so results are allocated without
-// the dispatcher, and several of one type at once.
+// the dispatcher, and the index tensors of a plan at once.
 Tensor new_tensor(c10::IntArrayRef sizes, c10::ScalarType type, const Tensor& on) {
   return at::detail::empty_cuda(sizes, type, on.device(), std::nullopt);
 }
@@ -209,9 +209,8 @@ std::tuple<Tensor, Tensor> cache4_read(Tensor cache, Tensor slots, std::optional
   const float* ks = check_scale(k_scale, cache, heads, "k_scale");
   const float* vs = check_scale(v_scale, cache, heads, "v_scale");
   const c10::cuda::CUDAGuard guard(cache.device());
-  const int64_t n = slots.size(0) * heads * D;
-  const Tensor all = new_tensor({2 * n}, dtype == 0 ? torch::kHalf : dtype == 1 ? torch::kBFloat16 : torch::kFloat32, cache);
-  Tensor k = part_of(all, 0, {slots.size(0), heads, D}), v = part_of(all, n, {slots.size(0), heads, D});
+  const auto type = dtype == 0 ? torch::kHalf : dtype == 1 ? torch::kBFloat16 : torch::kFloat32;
+  Tensor k = new_tensor({slots.size(0), heads, D}, type, cache), v = new_tensor({slots.size(0), heads, D}, type, cache);
   check_status(gfx906_b200_cache4_read(cache.data_ptr(), pages, slots.data_ptr<int>(), ks, vs,
                                        static_cast<int>(slots.size(0)), heads, D, k.data_ptr(), v.data_ptr(),
                                        static_cast<int>(dtype), at::cuda::getCurrentCUDAStream()));

@@ -329,3 +329,10 @@ def test_out_shares_no_row_with_other_rows_of_q():
     out = view(0, row, D)
     g.attn_cache4(spread, *args, out=out)
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_keys_and_values_read_have_memory_of_their_own(dtype):
+    cache, _, _, _ = held(*(torch.randn(7, 3, 64).half() for _ in range(2)))
+    for x in g.cache4_read(cache, ints(range(7)), dtype=dtype):
+        assert x.untyped_storage().nbytes() == 7 * 3 * 64 * dtype.itemsize and x.storage_offset() == 0
