@@ -241,13 +241,14 @@ struct Work {
   int r, block, head;   // r < 0: nothing
   int piece, most;      // piece of at most `most`
   int tail;             // number of the unit among those that are cut
+  int slot0;            // its first piece's slot in the workspace
 };
 // The same with what follows from it, in shared memory.
 struct Seg {
   int r, head, row0;     // request, kv head, first of its query rows
   int first, n, len;     // of the request
   int t0, t1;            // tiles of 128 keys
-  int tail, piece, pieces;
+  int tail, slot0, piece, pieces;
 };
 __device__ __forceinline__ int many_blocks(const ManyParams& p, int r) {
   const Rows t = rows_of(p.a, r);
@@ -286,7 +287,7 @@ __device__ __forceinline__ Work find_work(const ManyParams& p) {
     for (int i = 0; i < M_THREADS / 32; ++i) blocks += part[i];
     __syncthreads();
   }
-  Work out{-1, 0, 0, 0, 1, 0};
+  Work out{-1, 0, 0, 0, 1, 0, 0};
   if (blocks > p.max_units / p.a.kv_heads) return out;  // query_start decreases somewhere
   const int units = static_cast<int>(blocks) * p.a.kv_heads;
   const int tail = units % p.sms, whole = units - tail;
@@ -303,6 +304,7 @@ __device__ __forceinline__ Work find_work(const ManyParams& p) {
     const int i = unit - whole;
     out.tail = i / out.most;
     out.piece = i % out.most;
+    out.slot0 = i - out.piece;
     unit = whole + out.tail;
   } else {
     out.most = 1;
@@ -359,8 +361,8 @@ __device__ __forceinline__ Work find_work(const ManyParams& p) {
 
 // One row of the pieces of a unit, added in their order.
 template <int D, bool BF16>
-__device__ __forceinline__ void join_row(const ManyParams& p, int tail, int pieces, int row, int head, uint16_t* out) {
-  const long long slot0 = static_cast<long long>(tail) * MAX_PIECES;
+__device__ __forceinline__ void join_row(const ManyParams& p, long long slot0, int pieces, int row, int head,
+                                         uint16_t* out) {
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot0 * 2 * M_ROWS + row;
   float m = -INFINITY, l = 0.f;
   for (int k = 0; k < pieces; ++k) m = fmaxf(m, __ldcg(ml + k * 2 * M_ROWS).x);
@@ -499,7 +501,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
     if (u.piece >= pieces) return;
     if (threadIdx.x == 0) {
       sg = {u.r, u.head, row0, rows.first, rows.n, len, tiles * u.piece / pieces, tiles * (u.piece + 1) / pieces,
-            u.tail, u.piece, pieces};
+            u.tail, u.slot0, u.piece, pieces};
       for (int i = 0; i < 2 && pieces > 1; ++i) {  // set up the unit's counts, long before they are needed
         unsigned long long* count = p.done + u.tail * 2 + i;
         const unsigned long long was = *reinterpret_cast<volatile unsigned long long*>(count);
@@ -796,7 +798,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
       } else {
         // a piece: unnormalised O, m and l to the workspace, chunk-major (4 columns
         // of one row are 16 bytes, the 256 rows of a chunk are contiguous)
-        const long long slot = static_cast<long long>(sg.tail) * MAX_PIECES + sg.piece;
+        const long long slot = sg.slot0 + sg.piece;
         *reinterpret_cast<float2*>(p.part_ml + (slot * 2 * M_ROWS + at.tile * M_ROWS + at.row) * 2) = make_float2(m, l);
         if (some) {
           float* dst = p.part_o + slot * 2 * M_ROWS * D + (at.tile * M_ROWS + at.row) * 4;
@@ -828,7 +830,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
         met = met && tile_wait(C::B_WG, 1);
         if (met && last_flag[at.tile] && at.live) {
           const int t = a.token_of(at.my_row);
-          join_row<D, BF16>(p, sg.tail, sg.pieces, at.tile * M_ROWS + at.row, sg.head,
+          join_row<D, BF16>(p, sg.slot0, sg.pieces, at.tile * M_ROWS + at.row, sg.head,
                             a.o + (sg.first + t) * a.o_stride_t +
                                 (static_cast<long long>(sg.head + 1) * a.group + at.my_row - (t + 1) * a.group) * a.o_stride_h);
         }
@@ -850,8 +852,9 @@ ManyPlan many_plan(int tokens, int requests, int group, int kv_heads, int D, int
   if (blocks * kv_heads > INT_MAX - CUT_CTAS * sms) return pl;  // CTAs of a launch
   pl.fits = true;
   pl.max_units = static_cast<int>(blocks * kv_heads);
-  // cut units: fewer than SMs
-  const size_t rows = static_cast<size_t>(pl.max_units < sms ? pl.max_units : sms) * MAX_PIECES * 2 * M_ROWS;
+  // pieces of the units that are cut, fewer than SMs (find_work): 58 MB at D = 128
+  const int cut = pl.max_units < sms ? pl.max_units : sms;
+  const size_t rows = static_cast<size_t>(cut * MAX_PIECES < CUT_CTAS * sms ? cut * MAX_PIECES : CUT_CTAS * sms) * 2 * M_ROWS;
   pl.ml_off = rows * D * sizeof(float);
   pl.done_off = pl.ml_off + rows * 2 * sizeof(float);
   pl.done_words = sms * 2;

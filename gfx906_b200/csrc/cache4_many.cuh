@@ -12,8 +12,9 @@ struct ManyParams {
   int min_rows;      // requests with at most this many query rows are another kernel's
   int max_units;     // units of 256 query rows and a kv head, at most
   int sms;
-  float* part_o;     // [sms][MAX_PIECES][D / 4][256][4]
-  float* part_ml;    // [sms][MAX_PIECES][256][2]
+  // a slot for every piece that there can be, at most CUT_CTAS * sms
+  float* part_o;     // [slots][D / 4][256][4]
+  float* part_ml;    // [slots][256][2]
   // [sms][2] pieces of a cut unit that are in the workspace, for each of its query
   // tiles, tagged with the launch as in the other kernel. That kernel, which ends
   // every call, clears them: a CTA whose wait ran out does not count its piece, and

@@ -178,7 +178,7 @@ def test_attention_of_many_requests_with_wide_tables(hint):
         check_rows(out[r:r + 1], q[r:r + 1], k[:lengths[r]], v[:lengths[r]], 0.125, True, [0], [0, 13, 31], 1)
 
 
-def c_call(q, out, cache, tables, lengths, query_start, scale, causal=True):
+def c_call(q, out, cache, tables, lengths, query_start, scale, causal=True, workspace=None):
     """(run, workspace) of one attention call through the C ABI on the current stream, which `run` launches."""
     lib = CABI(build.LIB_PATH)
     a = Cache4AttnArgs(q=q.data_ptr(), o=out.data_ptr(), cache=cache.data_ptr(), tables=tables.data_ptr(),
@@ -187,7 +187,9 @@ def c_call(q, out, cache, tables, lengths, query_start, scale, causal=True):
                        dtype=int(q.dtype == torch.bfloat16), tokens=q.shape[0], heads=q.shape[1],
                        kv_heads=cache.shape[1], D=q.shape[2], pages=cache.shape[0], requests=tables.shape[0],
                        width=tables.shape[1], max_tokens=q.shape[0], causal=int(causal), zero_rest=1, scale=scale)
-    ws = torch.empty(lib.dll.gfx906_b200_cache4_attn_workspace_size(ctypes.byref(a)), dtype=torch.uint8, device="cuda")
+    bytes_ = lib.dll.gfx906_b200_cache4_attn_workspace_size(ctypes.byref(a))
+    ws = torch.empty(bytes_, dtype=torch.uint8, device="cuda") if workspace is None else workspace
+    assert ws.numel() == bytes_ and ws.data_ptr() % 256 == 0
 
     def run():
         rc = lib.dll.gfx906_b200_cache4_attn(ctypes.byref(a), ws.data_ptr(), ws.numel(),
@@ -336,3 +338,22 @@ def test_keys_and_values_read_have_memory_of_their_own(dtype):
     cache, _, _, _ = held(*(torch.randn(7, 3, 64).half() for _ in range(2)))
     for x in g.cache4_read(cache, ints(range(7)), dtype=dtype):
         assert x.untyped_storage().nbytes() == 7 * 3 * 64 * dtype.itemsize and x.storage_offset() == 0
+
+
+@pytest.mark.parametrize("requests,heads", [(1, 1), (1, 7), (30, 5), (49, 3), (21, 7), (100, 4)])
+def test_workspace_is_bounded_and_kept_to(requests, heads):
+    """Units of many rows that are cut in 2 to 16 pieces: at most three pieces an SM, 256 rows of sums each."""
+    n, rows, D, gen = 2300, 70, 128, torch.Generator().manual_seed(9)
+    cache, table, _, _ = held(*(torch.randn(n, heads, D, generator=gen).half() for _ in range(2)))
+    q = torch.randn(requests * rows, heads, D, generator=gen).half().cuda()
+    args = (cache, table.expand(requests, -1).contiguous(), ints([n - 13 * r for r in range(requests)]),
+            ints(range(0, requests * rows + 1, rows)), 0.09)
+    want, out = g.attn_cache4(q, *args), torch.empty_like(q)
+    run, ws = c_call(q, out, *args)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    few = sms * 3 * 2 * 16 * (D + 2) * 4  # sums of the other kernel's pieces: 16 rows, two a block
+    assert ws.numel() <= 3 * sms * 256 * (D + 2) * 4 + few + 65536
+    memory = torch.full((ws.numel() + 2 ** 20,), 0xa5, dtype=torch.uint8, device="cuda")
+    run, _ = c_call(q, out, *args, workspace=memory[:ws.numel()])
+    run()
+    assert torch.equal(out, want) and (memory[ws.numel():] == 0xa5).all()
