@@ -868,8 +868,11 @@ static Plan plan_of(const gfx906_b200_cache4_attn_args& g, int sms) {
   pl.ml_off = slots * g.D * sizeof(float);
   pl.done_off = pl.ml_off + slots * 2 * sizeof(float);
   pl.many_off = (pl.done_off + pl.blocks * sizeof(unsigned long long) + 255) & ~static_cast<size_t>(255);
+  // of all requests, so many can have more than FEW_ROWS rows
+  const long long large = static_cast<long long>(g.tokens) * (g.heads / g.kv_heads) / (FEW_ROWS + 1);
   if (rows > FEW_ROWS && g.requests > 0) {
-    pl.many = many_plan(g.tokens, g.requests, g.heads / g.kv_heads, g.kv_heads, g.D, sms);
+    pl.many = many_plan(g.tokens, static_cast<int>(min(large, static_cast<long long>(g.requests))), g.heads / g.kv_heads,
+                        g.kv_heads, g.D, sms);
     pl.fits = pl.fits && pl.many.fits;
   }
   pl.bytes = pl.many_off + ((pl.many.bytes + 255) & ~static_cast<size_t>(255));

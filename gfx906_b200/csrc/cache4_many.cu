@@ -846,6 +846,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
 }
 
 // -------------------------------------------------------------------- host
+// requests: those that can have rows for this kernel.
 ManyPlan many_plan(int tokens, int requests, int group, int kv_heads, int D, int sms) {
   ManyPlan pl{};
   const long long blocks = static_cast<long long>(tokens) * group / (2 * M_ROWS) + requests;

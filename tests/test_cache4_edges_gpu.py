@@ -357,3 +357,16 @@ def test_workspace_is_bounded_and_kept_to(requests, heads):
     run, _ = c_call(q, out, *args, workspace=memory[:ws.numel()])
     run()
     assert torch.equal(out, want) and (memory[ws.numel():] == 0xa5).all()
+
+
+def test_calls_without_a_hint_are_sized_by_the_rows_there_are():
+    """64 rows of four heads make three requests of more than 64 rows at most: four units, 16 pieces of each."""
+    cache, table, _, _ = held(*(torch.randn(100, 1, 128).half() for _ in range(2)))
+    q = torch.randn(64, 4, 128).half().cuda()
+    args = (cache, table.expand(64, -1).contiguous(), ints([100] * 64), ints(range(65)), 0.09)
+    out = torch.empty_like(q)
+    run, ws = c_call(q, out, *args)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert ws.numel() <= 4 * 16 * 256 * (128 + 2) * 4 + sms * 3 * 2 * 16 * (128 + 2) * 4 + 65536
+    run()
+    assert torch.equal(out, g.attn_cache4(q, *args))
