@@ -69,8 +69,6 @@ struct FewParams {
   unsigned long long* done;
   unsigned long long epoch;
   unsigned long long timeout_ns;
-  unsigned long long* many_done;  // the other kernel's counts, cleared here
-  int many_words;                 // 0: it was not launched
 };
 
 template <int D, int NT>
@@ -821,7 +819,6 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
     fa::fence_proxy_async_smem();  // what was stored in the rings comes before the next copies
     __syncthreads();               // the merge buffers, Q and row factors are free
   }
-  for (int i = blockIdx.x * THREADS + threadIdx.x; i < p.many_words; i += gridDim.x * THREADS) p.many_done[i] = 0;
   if (a.zero_rest) {
     const int from = min(max(a.query_start[a.requests], 0), a.tokens);
     const long long per = static_cast<long long>(a.kv_heads) * a.group * (D / 4);
@@ -926,8 +923,6 @@ static int attn(const gfx906_b200_cache4_attn_args& g, void* ws, size_t ws_bytes
     m.done = reinterpret_cast<unsigned long long*>(base + pl.many_off + pl.many.done_off);
     m.epoch = gfx906_b200_internal_next_epoch() & 0xffffffffffffull;
     m.timeout_ns = gfx906_b200_internal_timeout_ns();
-    p.many_done = m.done;
-    p.many_words = pl.many.done_words;
     const int st = launch_many(m, g.D, g.dtype, stream);
     if (st != GFX906_B200_OK) return st;
   }

@@ -258,6 +258,7 @@ __device__ __forceinline__ int many_blocks(const ManyParams& p, int r) {
 constexpr int MAX_PIECES = 16;
 constexpr int CUT_CTAS = 3;   // times the SMs: pieces of all units that are cut, at most
 constexpr int MIN_TILES = 4;  // of 128 keys, in a piece
+constexpr int LOST = 0x8000;  // in a unit's count: a piece did not come
 
 // All threads of the CTA. Units are numbered from the longest request down (up
 // to SORTED requests; their loads differ most where they are few), of one request
@@ -754,9 +755,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
       }
       const Place at(sg, a);
       const uint32_t tO = tS + 256 - at.tile * (128 - D);
-      if (!(st & OK)) {
-        // a wait ran out: nothing is stored
-      } else if (sg.pieces == 1) {
+      if (sg.pieces == 1 && (st & OK)) {
         // through this warp's staging tile, so that 8 lanes store 128 contiguous bytes of a row
         const float inv = m == -INFINITY ? 0.f : (a.v_scale ? a.v_scale[sg.head] : 1.f) / l;
         uint16_t* const o_head = a.o + sg.first * a.o_stride_t + static_cast<long long>(sg.head) * a.group * a.o_stride_h;
@@ -795,39 +794,50 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
           }
           __syncwarp();
         }
-      } else {
+      }
+      if (sg.pieces > 1) {
         // a piece: unnormalised O, m and l to the workspace, chunk-major (4 columns
         // of one row are 16 bytes, the 256 rows of a chunk are contiguous)
-        const long long slot = sg.slot0 + sg.piece;
-        *reinterpret_cast<float2*>(p.part_ml + (slot * 2 * M_ROWS + at.tile * M_ROWS + at.row) * 2) = make_float2(m, l);
-        if (some) {
-          float* dst = p.part_o + slot * 2 * M_ROWS * D + (at.tile * M_ROWS + at.row) * 4;
+        bool met = st & OK;
+        if (met) {
+          const long long slot = sg.slot0 + sg.piece;
+          *reinterpret_cast<float2*>(p.part_ml + (slot * 2 * M_ROWS + at.tile * M_ROWS + at.row) * 2) = make_float2(m, l);
+          if (some) {
+            float* dst = p.part_o + slot * 2 * M_ROWS * D + (at.tile * M_ROWS + at.row) * 4;
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(tO + 32 * c, o);
-            tmem_wait_ld();
-            reg_fence32(o);
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tO + 32 * c, o);
+              tmem_wait_ld();
+              reg_fence32(o);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              *reinterpret_cast<float4*>(dst + (c * 8 + e) * 2 * M_ROWS * 4) =
-                  make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
-                              __uint_as_float(o[4 * e + 3]));
+              for (int e = 0; e < 8; ++e)
+                *reinterpret_cast<float4*>(dst + (c * 8 + e) * 2 * M_ROWS * 4) =
+                    make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
+                                __uint_as_float(o[4 * e + 3]));
+            }
           }
+          // The rendezvous orders the warpgroup's stores before one thread's
+          // fence, and that before its count.
+          mbar_arrive(bar + 8 * C::B_WG);
+          met = tile_wait(C::B_WG, 0);
         }
-        // The rendezvous orders the warpgroup's stores before one thread's
-        // fence, and that before its count.
-        mbar_arrive(bar + 8 * C::B_WG);
-        bool met = tile_wait(C::B_WG, 0);
-        if (met && at.row == 0) {
+        if (at.row == 0) {
           unsigned long long* count = p.done + sg.tail * 2 + at.tile;
+          if (!met) atomicOr(count, static_cast<unsigned long long>(LOST));
           __threadfence();
-          const bool last = static_cast<int>(atomicAdd(count, 1ull) & 0xffffull) + 1 == sg.pieces;
-          if (last) __threadfence();
-          last_flag[at.tile] = last;
+          const int before = static_cast<int>(atomicAdd(count, 1ull) & 0xffffull);
+          const bool last = (before & ~LOST) + 1 == sg.pieces;
+          if (last) {
+            __threadfence();
+            atomicExch(count, p.epoch << 16);
+          }
+          last_flag[at.tile] = last && !(before & LOST);
         }
-        mbar_arrive(bar + 8 * C::B_WG);
-        met = met && tile_wait(C::B_WG, 1);
+        if (met) {
+          mbar_arrive(bar + 8 * C::B_WG);
+          met = tile_wait(C::B_WG, 1);
+        }
         if (met && last_flag[at.tile] && at.live) {
           const int t = a.token_of(at.my_row);
           join_row<D, BF16>(p, sg.slot0, sg.pieces, at.tile * M_ROWS + at.row, sg.head,
@@ -858,8 +868,7 @@ ManyPlan many_plan(int tokens, int requests, int group, int kv_heads, int D, int
   const size_t rows = static_cast<size_t>(cut * MAX_PIECES < CUT_CTAS * sms ? cut * MAX_PIECES : CUT_CTAS * sms) * 2 * M_ROWS;
   pl.ml_off = rows * D * sizeof(float);
   pl.done_off = pl.ml_off + rows * 2 * sizeof(float);
-  pl.done_words = sms * 2;
-  pl.bytes = pl.done_off + pl.done_words * sizeof(unsigned long long);
+  pl.bytes = pl.done_off + static_cast<size_t>(sms) * 2 * sizeof(unsigned long long);
   return pl;
 }
 

@@ -16,9 +16,9 @@ struct ManyParams {
   float* part_o;     // [slots][D / 4][256][4]
   float* part_ml;    // [slots][256][2]
   // [sms][2] pieces of a cut unit that are in the workspace, for each of its query
-  // tiles, tagged with the launch as in the other kernel. That kernel, which ends
-  // every call, clears them: a CTA whose wait ran out does not count its piece, and
-  // a replay of the launch, which has the same tag, must not find what is left.
+  // tiles, tagged with the launch as in the other kernel. A CTA whose wait ran out
+  // counts its piece too, as LOST: the unit is not joined then, and its word is
+  // none again for a replay of the launch, which has the same tag.
   unsigned long long* done;
   unsigned long long epoch;
   unsigned long long timeout_ns;
@@ -27,7 +27,6 @@ struct ManyPlan {
   bool fits;      // false: too large a call
   int max_units;
   size_t ml_off, done_off, bytes;  // workspace
-  int done_words;
 };
 ManyPlan many_plan(int tokens, int requests, int group, int kv_heads, int D, int sms);
 int launch_many(const ManyParams& p, int D, int dtype, cudaStream_t stream);

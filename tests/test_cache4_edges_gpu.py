@@ -199,8 +199,9 @@ def c_call(q, out, cache, tables, lengths, query_start, scale, causal=True, work
 
 
 def test_no_count_of_a_launch_is_left_for_its_replay():
-    """Pieces of many rows are counted in the workspace's last words under the launch's tag, which a replayed graph
-    keeps. A CTA whose wait runs out does not count; were a partial count left, every replay would join too early."""
+    """Pieces of many rows are counted in the workspace's last words, two to an SM, under the launch's tag, which a
+    replayed graph keeps. A CTA whose wait runs out marks its unit's word (bit 15): that unit is not joined, and the
+    next replay finds nothing of it."""
     n, rows, gen = 4500, 600, torch.Generator().manual_seed(6)
     cache, table, k, v = held(*(torch.randn(n, 1, 64, generator=gen).half() for _ in range(2)))
     q = torch.randn(rows, 1, 64, generator=gen).half().cuda()
@@ -208,16 +209,24 @@ def test_no_count_of_a_launch_is_left_for_its_replay():
     want, out = g.attn_cache4(q, *args), torch.empty_like(q)
     run, ws = c_call(q, out, *args)
     sms = torch.cuda.get_device_properties(0).multi_processor_count
-    words = ws[-(-(-16 * sms // 256) * 256):].view(torch.int64)[:2 * sms]  # two to an SM, the region a multiple of 256 bytes
-    ws.fill_(0x5a)
+    words = ws[-(-(-16 * sms // 256) * 256):].view(torch.int64)[:2 * sms]  # the region is a multiple of 256 bytes
+    ws.fill_(0)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         run()
-    for _ in range(3):
+    for lost in (None, 0, None, 3, None, None):
+        if lost is not None:
+            assert words[lost]  # tagged by the launch before
+            words[lost] |= 0x8000
         out.fill_(7)
         graph.replay()
         torch.cuda.synchronize()
-        assert torch.equal(out, want) and not words.any()
+        assert not (words & 0xffff).any()
+        stored = (out == want).flatten(1).all(1)
+        if lost is None:
+            assert stored.all()
+        else:  # one tile of 128 rows of a unit of 256, as it was
+            assert int((~stored).sum()) in (128, rows % 256 % 128) and (out[~stored] == 7).all()
 
 
 SHORT_WAITS = """
