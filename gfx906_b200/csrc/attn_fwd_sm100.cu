@@ -81,6 +81,10 @@ constexpr int PRODUCER_WARP = 8;
 constexpr int MMA_WARP = 9;
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units
 constexpr int MAX_PIECES = 32;             // most pieces one split unit is cut into
+#ifndef ATTN_EMU_PAIRS
+#define ATTN_EMU_PAIRS 1
+#endif
+constexpr int EMU_PAIRS = ATTN_EMU_PAIRS;  // see row_exp_store
 // Roles recorded in the timeout diagnostics.
 enum Role : int { ROLE_PRODUCER = 1, ROLE_MMA = 2, ROLE_SOFTMAX0 = 3, ROLE_SOFTMAX1 = 4 };
 
@@ -703,9 +707,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const uint32_t half_bar = bars + 8 * (C::B_P_HALF + ti);
         float lsum0, lsum1;
         if (full)
-          row_exp_store<false>(s, sl2, neg_m, nvalid, tP, lsum0, lsum1, half_bar, [] {}, before_store);
+          row_exp_store<EMU_PAIRS, false>(s, sl2, neg_m, nvalid, tP, lsum0, lsum1, half_bar, [] {}, before_store);
         else
-          row_exp_store<true>(s, sl2, neg_m, nvalid, tP, lsum0, lsum1, half_bar, [] {}, before_store);
+          row_exp_store<EMU_PAIRS, true>(s, sl2, neg_m, nvalid, tP, lsum0, lsum1, half_bar, [] {}, before_store);
         l_run += lsum0 + lsum1;
         tmem_wait_st();
         tc_fence_before();
@@ -1254,9 +1258,9 @@ __global__ void __launch_bounds__(Cfg512P::THREADS, 1)
         l_run *= factor;
         float lsum0, lsum1;
         if (full)
-          row_exp_store<false>(s, sl2, -m_run, nvalid, tS, lsum0, lsum1, 0u, [] {}, [] {});
+          row_exp_store<EMU_PAIRS, false>(s, sl2, -m_run, nvalid, tS, lsum0, lsum1, 0u, [] {}, [] {});
         else
-          row_exp_store<true>(s, sl2, -m_run, nvalid, tS, lsum0, lsum1, 0u, [] {}, [] {});
+          row_exp_store<EMU_PAIRS, true>(s, sl2, -m_run, nvalid, tS, lsum0, lsum1, 0u, [] {}, [] {});
         l_run += lsum0 + lsum1;
         // O may only be rescaled once PV(j-1) has completed.
         if (j > t0) {

@@ -11,12 +11,6 @@
 namespace fa {
 
 constexpr int BN = 128;  // keys per K/V tile = columns of a score row
-#ifndef ATTN_EMU_PAIRS
-#define ATTN_EMU_PAIRS 1
-#endif
-// Pairs of exponentials, out of every 4 pairs (8 columns), evaluated with the
-// FMA-pipe polynomial instead of MUFU ex2 (balances the two pipes).
-constexpr int EMU_PAIRS = ATTN_EMU_PAIRS;
 
 // Max over the valid columns [lo, nvalid) of a raw score row (min when the scale is
 // negative), so that extreme * scale is the row max of the scaled scores.
@@ -59,7 +53,7 @@ __device__ __forceinline__ float row_extreme(const uint32_t* s, int nvalid, bool
 // P = exp2(s * sl2 + neg_m) for one 128-column score row, rounded to fp16 and
 // stored into TMEM columns [tS, tS + 64) (two fp16 per column); returns the
 // fp32 row sum in two partial sums. EMU_PAIRS of every 4 column pairs use the
-// FMA-pipe polynomial, the rest MUFU. MASK zeroes columns outside [lo,
+// FMA-pipe polynomial, the rest MUFU (balances the two pipes). MASK zeroes columns outside [lo,
 // nvalid) (last key tile).
 // TWO_STEPS rounds the product before neg_m is added, as a maximum that was
 // computed by itself was rounded.
@@ -67,7 +61,7 @@ __device__ __forceinline__ float row_extreme(const uint32_t* s, int nvalid, bool
 // it as soon as it is stored (after before_half() has run), so the tensor core
 // can start on those keys while the second half is computed. before_store()
 // runs once, after the first half's exponentials and before any of P is stored.
-template <bool MASK, bool TWO_STEPS = false, typename BeforeHalf, typename BeforeStore>
+template <int EMU_PAIRS, bool MASK, bool TWO_STEPS = false, typename BeforeHalf, typename BeforeStore>
 __device__ __forceinline__ void row_exp_store(const uint32_t* s, float sl2, float neg_m, int nvalid,
                                               uint32_t tS, float& sum0, float& sum1, uint32_t half_bar,
                                               BeforeHalf&& before_half, BeforeStore&& before_store, int lo = 0) {

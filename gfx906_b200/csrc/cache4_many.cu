@@ -31,10 +31,6 @@
 #include <limits.h>
 #include <math.h>
 
-// All exponentials on MUFU here, none by polynomial: the conversions already
-// keep the FMA pipe busy (4096 rows x 24 heads against 16384 keys: 775 us; with
-// one pair in four on the FMA pipe, as the dense kernels have it, 793; two, 899).
-#define ATTN_EMU_PAIRS 0
 #include "attn_row.cuh"
 #include "cache4.cuh"
 #include "cache4_attn.cuh"
@@ -58,6 +54,10 @@ constexpr int BOX = 16384;           // 128 rows x 64 fp16 columns, 128-byte swi
 constexpr uint32_t M_REGS_SOFTMAX = 184;
 constexpr uint32_t M_REGS_CONVERT = 64;
 constexpr uint32_t M_REGS_ISSUE = 80;
+// All exponentials on MUFU here, none by polynomial: the conversions already
+// keep the FMA pipe busy (4096 rows x 24 heads against 16384 keys: 775 us; with
+// one pair in four on the FMA pipe, as the dense kernels have it, 793; two, 899).
+constexpr int M_EMU_PAIRS = 0;
 constexpr float M_RESCALE = 8.0f;    // log2 units, see the dense kernels
 // A row's reference m is set this far below its largest score, so that P, which
 // stays below 2^(M_HEAD + M_RESCALE), uses all of fp16's range: weights down to
@@ -739,9 +739,9 @@ __global__ void __launch_bounds__(M_THREADS, 1) cache4_many_kernel(const ManyPar
         // Where scores are so large that m is a rounded product, each score is
         // rounded as m was, or the largest would lie half a step of m off it.
         if (full && !(st & LARGE))
-          row_exp_store<false>(s, sl2, neg_m, hi, tS, sum0, sum1, bar + 8 * C::B_P_HALF, [] {}, [] {});
+          row_exp_store<M_EMU_PAIRS, false>(s, sl2, neg_m, hi, tS, sum0, sum1, bar + 8 * C::B_P_HALF, [] {}, [] {});
         else
-          row_exp_store<true, true>(s, sl2, neg_m, hi, tS, sum0, sum1, bar + 8 * C::B_P_HALF, [] {}, [] {}, lo);
+          row_exp_store<M_EMU_PAIRS, true, true>(s, sl2, neg_m, hi, tS, sum0, sum1, bar + 8 * C::B_P_HALF, [] {}, [] {}, lo);
         l += sum0 + sum1;
         tmem_wait_st();
         tc_fence_before();
