@@ -651,9 +651,8 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
         uint4 x = q[i];
         float f = 1.f;
         if (BF16) {
-          // bf16 rows are scaled by a power of two that brings their largest
-          // number to [1, 2) and then fit fp16: what falls below 2^-24 of the
-          // largest is lost, less than the 32-bit sums keep
+          // into fp16 (row_exponent): numbers below 2^-14 of the row's largest are
+          // rounded by up to 2^-25 of it
           const uint32_t w[4] = {x.x, x.y, x.z, x.w};
           float y[8], mx = 0.f;
 #pragma unroll
@@ -665,13 +664,11 @@ __global__ void __launch_bounds__(Few<D, NT>::THREADS, Few<D, NT>::PER_SM) cache
           }
 #pragma unroll
           for (int d = PER_ROW / 2; d > 0; d /= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-          const uint32_t ex = (__float_as_uint(mx) >> 23) & 255u;
-          if (ex > 0 && ex < 254) {  // not for zeros, subnormal rows and infinities
-            f = __uint_as_float(ex << 23);
-            const float inv = __uint_as_float((254u - ex) << 23);
+          const uint32_t ex = row_exponent(mx);
+          f = __uint_as_float(ex << 23);
+          const float inv = __uint_as_float((254u - ex) << 23);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] *= inv;
-          }
+          for (int e = 0; e < 8; ++e) y[e] *= inv;
           x = make_uint4(fa::pack_half2(y[0], y[1]), fa::pack_half2(y[2], y[3]), fa::pack_half2(y[4], y[5]),
                          fa::pack_half2(y[6], y[7]));
         }

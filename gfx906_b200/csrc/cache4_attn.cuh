@@ -31,6 +31,16 @@ inline unsigned group_magic(long long rows, int group) {
   return group > 1 && rows * group < (1ll << 32) ? static_cast<unsigned>(((1ll << 32) + group - 1) / group) : 0u;
 }
 
+// Rows of bf16 are divided by a power of two that brings their largest number to
+// [1, 2) and then fit fp16; this is its exponent field, from that of the largest.
+// The first power stands for subnormal rows too, the last but one for the largest
+// rows, whose own reciprocal would be subnormal. Rows that hold an infinity or NaN
+// stay as they are (127: a power of one).
+__device__ __forceinline__ uint32_t row_exponent(float largest) {
+  const uint32_t ex = (__float_as_uint(largest) >> 23) & 255u;
+  return ex == 255u ? 127u : min(max(ex, 1u), 253u);
+}
+
 // Query rows of request r: first token and number of tokens, whatever the
 // array holds (it comes from the caller's device memory).
 struct Rows {

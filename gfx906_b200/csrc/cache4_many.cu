@@ -405,10 +405,8 @@ __device__ __forceinline__ void join_row(const ManyParams& p, long long slot0, i
 
 // A warp's 32 rows of a query tile, from row0 on, into the swizzled layout of the
 // tensor core's A operand, whole rows per D / 8 lanes; rows behind the request's
-// last are zero. Rows of bf16 are
-// divided by a power of two that brings their largest number to [1, 2) and then
-// fit fp16 (what falls below 2^-24 of a row's largest is lost); rowf[row] keeps
-// its exponent.
+// last are zero. Rows of bf16 go into fp16 (row_exponent; numbers below 2^-14 of
+// the row's largest are rounded by up to 2^-25 of it); rowf[row] keeps the exponent.
 template <int D, bool BF16>
 __device__ __forceinline__ void put_q(const AttnParams& a, const Seg& sg, int tile0, int row0, int lane, uint32_t tile,
                                       uint8_t* rowf) {
@@ -438,15 +436,14 @@ __device__ __forceinline__ void put_q(const AttnParams& a, const Seg& sg, int ti
       }
 #pragma unroll
       for (int d = LANES / 2; d > 0; d /= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-      const uint32_t ex = (__float_as_uint(mx) >> 23) & 255u;
-      const bool scaled = ex > 0 && ex < 254;
-      const float inv = scaled ? __uint_as_float((254u - ex) << 23) : 1.f;
+      const uint32_t ex = row_exponent(mx);
+      const float inv = __uint_as_float((254u - ex) << 23);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 f = bf162_to_float2(w[e]);
         w[e] = pack_half2(f.x * inv, f.y * inv);
       }
-      if (ch == 0) rowf[row] = static_cast<uint8_t>(scaled ? ex : 127u);
+      if (ch == 0) rowf[row] = static_cast<uint8_t>(ex);
       st_shared_v4(place(row), w[0], w[1], w[2], w[3]);
     }
   }

@@ -379,3 +379,18 @@ def test_calls_without_a_hint_are_sized_by_the_rows_there_are():
     assert ws.numel() <= 4 * 16 * 256 * (128 + 2) * 4 + sms * 3 * 2 * 16 * (128 + 2) * 4 + 65536
     run()
     assert torch.equal(out, g.attn_cache4(q, *args))
+
+
+@pytest.mark.parametrize("rows", [1, 12, 130])
+@pytest.mark.parametrize("power", [127, 126, -125, -126, -127, -130])
+def test_the_largest_and_smallest_rows_of_bf16(power, rows):
+    """Rows whose largest number is next to bf16's largest, or subnormal, under a factor that makes up for it."""
+    n, D, gen = 300, 64, torch.Generator().manual_seed(10)
+    cache, table, k, v = held(*(torch.randn(n, 1, D, generator=gen).half() for _ in range(2)))
+    factor = 2.0 ** (-power if power > 0 else min(-power, 127))
+    x = torch.randn(rows, 1, D, generator=gen)
+    x = (x / x.abs().amax(-1, keepdim=True) * 1.9 * 2.0 ** power).to(torch.bfloat16)
+    assert x.isfinite().all() and x.any()
+    out = g.attn_cache4(x.cuda(), cache, table, ints([n]), ints([0, rows]), 1.0, causal=False, max_tokens=rows,
+                        k_scale=torch.tensor([factor], device="cuda"))
+    check_rows(out, x.double() * factor, k, v, 1.0, False, range(0, rows, 9), [0], 1)
