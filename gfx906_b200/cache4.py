@@ -20,8 +20,11 @@ waiting for the GPU::
         q, k, v = layer.project(x, plan.positions)
         cache4_write(k, v, layer.cache, plan.slots, layer.k_scale, layer.v_scale)
         o = attn_cache4(q, layer.cache, tables, plan.lengths, plan.query_start, scale,
-                        k_scale=layer.k_scale, v_scale=layer.v_scale)
+                        k_scale=layer.k_scale, v_scale=layer.v_scale, max_tokens=most)
     lengths, free_count = plan.lengths, plan.free_count
+
+where ``most`` is the largest of the counts, which the program that sets them
+knows.
 
 A number is an e2m1 code times an e4m3 scale, shared by 16 neighbouring
 channels of a token, times a float32 factor per kv head (``k_scale``,
@@ -30,7 +33,9 @@ leaves e4m3's range: the largest magnitude of a head divided by 2688 keeps all
 of it. The byte layout of a page is in ``csrc/cache4.cuh``.
 
 Every operator raises RuntimeError on arguments it does not take, runs on its
-tensors' device, and can be captured in a CUDA graph. Index tensors are int32.
+tensors' device, and can be captured in a CUDA graph; like ``attn`` they record
+no gradient. ``set_sm_limit`` does not hold for them: their blocks are many and
+short, and go to any SM that is free. Index tensors are int32.
 Page ids and slots come from device memory and are checked there: what lies
 outside the cache is skipped.
 """
@@ -92,8 +97,10 @@ def cache4_plan(tables, lengths, counts, free_pages, free_count, tokens):
 
     Pages of ended requests go back first and may be granted in the same step.
     Then requests get pages in their order; one is refused -- ``added`` 0, slots
-    -1, length unchanged -- when its tokens fit neither its row of tables nor
-    the buffer, or when the free pages do not cover it and all before it.
+    -1, length unchanged -- when its tokens do not fit its row of tables, when
+    they do not fit the buffer, or when the free pages do not cover it and all
+    before it. Tokens in a page whose id is negative or beyond 2^25 - 1 get slot
+    -1 as well.
     tables and free_pages are updated in place, only where the inputs do not
     use them: until lengths and free_count are replaced by the returned ones, a
     step may be planned again.
@@ -115,7 +122,8 @@ def cache4_write(k, v, cache, slots, k_scale=None, v_scale=None):
 def cache4_read(cache, slots, k_scale=None, v_scale=None, dtype=torch.float16):
     """The keys and values at ``slots`` [tokens] as two contiguous tensors
     [tokens, kv_heads, head_dim] of fp16, bf16 or fp32; zeros where a slot lies
-    outside the cache (-1)."""
+    outside the cache (-1). What a number was rounded up to in the cache may lie
+    beyond fp16's range (6% at most for fp16 keys and values) and is then infinite."""
     if dtype not in _READ_DTYPES:
         raise RuntimeError("cache4: dtype must be float16, bfloat16 or float32")
     return _module().cache4_read(cache, slots, k_scale, v_scale, _READ_DTYPES[dtype])
@@ -135,8 +143,15 @@ def attn_cache4(q, cache, tables, lengths, query_start, scale, causal=True, k_sc
     less; without, every row sees them all. Rows that see none are zero.
 
     max_tokens: no request has more rows than this, if known; it chooses the
-    kernels (default: all rows of q may be one request's). Too small a value
-    costs time, not correctness. Returns a new tensor, with zeros in rows behind
+    kernels (default: all rows of q may be one request's, which costs a step of
+    64 single tokens half its time again). Too small a value costs time, not
+    correctness.
+
+    Scores, softmax sums and the output are held in 32 bits, and the output is
+    rounded once. Weights are rounded to fp16 on their way to the tensor core:
+    by 2^-11 of themselves down to 2^-21 of a row's largest, below that by 2^-32
+    of it. Rows of bf16 go into fp16 divided by a power of two; their numbers
+    below 2^-14 of the row's largest are rounded by up to 2^-25 of it. Returns a new tensor, with zeros in rows behind
     the last request, or ``out``, whose rows behind the last request are left
     as they were. ``out`` is q itself, or shares no row with q and no memory
     with the other arguments.

@@ -23,11 +23,13 @@
 // per pair, in registers.
 //
 // Measured (B200, D = 128, 8 kv heads of 4 query heads): 32 requests of up to
-// 16384 tokens 79 us, 4.7 TB/s of cache; 131072 tokens of one request 40 us, 3.7
-// TB/s. With the arithmetic taken out the same copies take 69 and 35 us, with the
-// copies taken out the arithmetic takes 74 and 40 (about 580 instructions of a
-// warp per step, 270 of them on the ALU pipe, 128 of these conversions): it is
-// bound by both, and by the 8 us before the first step and behind the last.
+// 16384 tokens 78 us in a captured graph, 4.7 TB/s of cache (84 us called with
+// other inputs each time); 131072 tokens of one request 41 us, 3.6 TB/s. No unit
+// is full (ALU pipe 53%, issue slots 59%, DRAM 53% of the time, 14 warps on an SM):
+// 3.5 warps a scheduler do not overlap copies with arithmetic. With the arithmetic
+// taken out the copies still take 69 and 35 us, with the copies taken out the
+// arithmetic 74 and 40 (about 580 instructions of a warp per step, 270 of them on
+// the ALU pipe); 8 us pass before the first step and behind the last.
 #include <limits.h>
 #include <math.h>
 
@@ -41,10 +43,12 @@ namespace c4 {
 
 // Requests with more query rows (tokens times heads of a group) go to the
 // tensor-memory kernel of cache4_many.cu, which takes 256 rows at the price of
-// one. Measured at D = 128, us here and there for 48, 64, 96, 128 rows a request:
-// 1 x 8192 keys, 8 kv heads: 30, 33, 36, 41 and 41, 41, 41, 43; 8 x 4096, 8: 53,
-// 64, 85, 106 and 52, 52, 52, 53; 32 x 2048, 8: 94, 119, 167, 213 and 124, 125,
-// 126, 130; 4 x 32768, 2: 52, 60, 80, 100 and 79, 78, 79, 80.
+// one. Measured, us here and there for 48, 64, 96, 128 rows a request:
+// D = 128: 1 x 8192 keys, 8 kv heads: 29, 31, 34, 38 and 38, 39, 39, 40; 8 x 4096,
+// 8: 50, 60, 81, 101 and 48, 48, 48, 49; 32 x 2048, 8: 87, 111, 154, 196 and 122,
+// 123, 125, 128; 4 x 32768, 2: 49, 56, 74, 93 and 72, 73, 74, 75.
+// D = 64: 23, 25, 25, 27 and 30, 30, 30, 31; 34, 39, 50, 64 and 42, 42, 42, 42; 56,
+// 70, 95, 121 and 92, 92, 92, 93; 34, 38, 49, 60 and 59, 60, 60, 61.
 constexpr int FEW_ROWS = 64;
 
 constexpr int MAX_REQUESTS = 8192;

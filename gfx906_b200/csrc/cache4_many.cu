@@ -24,10 +24,13 @@
 //
 // Measured (B200, D = 128): 4096 rows x 24 heads against 16384 keys 760 us, 1085
 // TFLOP/s, 0.66 of a library bf16 product's rate; four prompts of 511 to 1021
-// tokens behind up to 8192, 32 heads on 8, causal, 249 us. Per 128 keys the
-// tensor core needs 1100 cycles of the 3300 that pass; the rest is the chain
-// S -> softmax -> P -> next S of each tile, which two tiles hide in part only.
-// Tensor memory (S0, S1, O0, O1) leaves no room for a third.
+// tokens behind up to 8192, 32 heads on 8, causal, 249 us (803 TFLOP/s: its units
+// differ in length, and the last wave is cut by their number). Called back to back
+// for seconds, under the power cap, the former takes 820. Per 128 keys the
+// products are 2050 cycles of the tensor core (8192 operations a cycle) out of the
+// 4500 that pass at 1.84 to 1.97 GHz; the rest is the chain S -> softmax -> P ->
+// next S of each tile, which two tiles hide in part only. Tensor memory (S0, S1,
+// O0, O1) leaves no room for a third.
 #include <limits.h>
 #include <math.h>
 
@@ -255,16 +258,22 @@ __device__ __forceinline__ int many_blocks(const ManyParams& p, int r) {
   const int rows = t.n * p.a.group;
   return rows > p.min_rows ? (rows + 2 * M_ROWS - 1) / (2 * M_ROWS) : 0;
 }
-constexpr int MAX_PIECES = 16;
-constexpr int CUT_CTAS = 3;   // times the SMs: pieces of all units that are cut, at most
-constexpr int MIN_TILES = 4;  // of 128 keys, in a piece
+// Measured at D = 128, us for four prompts of up to 1021 tokens behind up to 8192
+// (8 x 4 heads) / 130 rows x 8 heads against 32768 keys / 100 requests of 70 to 300
+// tokens, up to 1000 keys (2 x 4 heads) / 4096 rows x 24 heads, causal, against
+// 16384: 275 / 68 / 124 / 482 with the numbers below.
+constexpr int MAX_PIECES = 16;  // 8: 275 / 73 / 124 / 482; 32: 275 / 68 / 124 / 482
+// Times the SMs: pieces of all units that are cut, at most. 2: 275 / 68 / 124 /
+// 460; 6: 276 / 68 / 138 / 484.
+constexpr int CUT_CTAS = 3;
+constexpr int MIN_TILES = 4;  // of 128 keys, in a piece; 2: 289 / 68 / 123 / 482; 8: 279 / 68 / 124 / 482
 constexpr int LOST = 0x8000;  // in a unit's count: a piece did not come
 
 // All threads of the CTA. Units are numbered from the longest request down (up
 // to SORTED requests; their loads differ most where they are few), of one request
 // from the last block down, which sees the most keys, the kv heads of a block one
-// after the other: what is dealt last is short. Four prompts: 249 us, in the
-// order of the requests 265.
+// after the other: what is dealt last is short. In the order of the requests the
+// cases above take 295 / 68 / 139 / 481 us.
 constexpr int SORTED = 128;
 __device__ __forceinline__ Work find_work(const ManyParams& p) {
   __shared__ int part[M_THREADS / 32];
@@ -293,7 +302,8 @@ __device__ __forceinline__ Work find_work(const ManyParams& p) {
   const int units = static_cast<int>(blocks) * p.a.kv_heads;
   const int tail = units % p.sms, whole = units - tail;
   // the number of pieces that ends the last wave soonest (a lane tries each),
-  // with a hundredth of a unit as the price of a piece
+  // with a hundredth of a unit as the price of a piece (a thousandth: 275 / 60 /
+  // 124 / 482, three: 275 / 85 / 124 / 482)
   const int pieces = lane % MAX_PIECES + 1;
   const int cost = pieces == 1 || tail * pieces <= CUT_CTAS * p.sms
                        ? (tail * pieces + p.sms - 1) / p.sms * 1000 / pieces + 10 * pieces

@@ -11,6 +11,8 @@
  * graphs. Status codes are those of gfx906_b200_attn.h. dtype: 0 = fp16,
  * 1 = bf16, 2 = fp32 (reads only). Strides are in elements; rows (the last
  * dimension) are contiguous, start on 16 bytes, and strides are multiples of 8.
+ * gfx906_b200_attn_set_sm_limit does not hold for these kernels: their blocks
+ * are many and short, and go to any SM that is free.
  */
 #ifndef GFX906_B200_CACHE4_H
 #define GFX906_B200_CACHE4_H
