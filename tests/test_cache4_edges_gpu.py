@@ -394,3 +394,23 @@ def test_the_largest_and_smallest_rows_of_bf16(power, rows):
     out = g.attn_cache4(x.cuda(), cache, table, ints([n]), ints([0, rows]), 1.0, causal=False, max_tokens=rows,
                         k_scale=torch.tensor([factor], device="cuda"))
     check_rows(out, x.double() * factor, k, v, 1.0, False, range(0, rows, 9), [0], 1)
+
+
+@pytest.mark.parametrize("sms", [1, 2, 7, 147])
+def test_attention_planned_for_fewer_sms(sms):
+    """A cap on the SMs of other kernels changes how the work is cut, not what comes out."""
+    n, H, D, gen = 1500, 2, 64, torch.Generator().manual_seed(11)
+    cache, table, k, v = held(*(torch.randn(n, H, D, generator=gen).half() for _ in range(2)))
+    counts = [1, 150, 0, 3, 300, 1]
+    starts = [sum(counts[:r]) for r in range(len(counts) + 1)]
+    lengths = [1500, 1400, 5, 3, 900, 0]
+    q = torch.randn(starts[-1], H, D, generator=gen).half()
+    with g.sm_limit(sms):
+        out = g.attn_cache4(q.cuda(), cache, table.expand(len(counts), -1).contiguous(), ints(lengths), ints(starts), 0.125)
+    for r, c in enumerate(counts):
+        rows = [i for i in (0, 1, 2, 77, 128, 149, 255, 256, 299) if i < c]
+        if lengths[r]:
+            check_rows(out[starts[r]:starts[r + 1]], q[starts[r]:starts[r + 1]], k[:lengths[r]], v[:lengths[r]], 0.125, True,
+                       rows, range(H), 1)
+        else:
+            assert not out[starts[r]:starts[r + 1]].any()
